@@ -18,7 +18,7 @@ import numpy as np
 LIB_PATH = Path(__file__).resolve().parent / "libkge_b200.so"
 
 OK, INVALID_ARGUMENT, RUNTIME_ERROR, DEVICE_STATUS, LOGIC_ERROR = range(5)
-F32, U32, F16 = 0, 1, 2
+F32, U32, F16, BF16 = 0, 1, 2, 3
 SET_STRING, SET_BOOL, SET_FLOAT, SET_UNSIGNED = 0, 1, 2, 3
 L1, L2, DOT = 0, 1, 2
 
@@ -32,6 +32,9 @@ SYMBOLS = (
     "kge_op_scatter_add_rows_noalloc", "kge_op_tc_gemm", "kge_op_tc_planes",
     "kge_microbench_rows", "kge_microbench_scores", "kge_op_tc_planes_bf16",
     "kge_op_activation", "kge_op_all_to_all",
+    "kge_op_log_probs_workspace", "kge_op_log_probs", "kge_op_log_probs_grad", "kge_op_rows8_bytes", "kge_op_quantise_rows",
+    "kge_op_product8_workspace", "kge_op_product8", "kge_op_product8_status", "kge_op_adamw", "kge_op_adamw_key",
+    "kge_op_adamw_moments",
 )
 
 
@@ -43,6 +46,29 @@ class Setting(C.Structure):
 class Array(C.Structure):
     _fields_ = [("name", C.c_char_p), ("dtype", C.c_int), ("rank", C.c_int),
                 ("shape", C.POINTER(C.c_size_t)), ("data", C.c_void_p)]
+
+
+class Scores(C.Structure):
+    """``kge_scores``; every pointer is a device address."""
+
+    _fields_ = [("x", C.c_void_p), ("float_type", C.c_int), ("rows", C.c_size_t), ("cols", C.c_size_t), ("row_stride", C.c_longlong),
+                ("mask", C.c_void_p), ("mask_stride", C.c_longlong), ("count", C.c_void_p), ("target", C.c_void_p), ("scale", C.c_float)]
+
+
+class LogProbsOut(C.Structure):
+    _fields_ = [("log_prob", C.c_void_p), ("entropy", C.c_void_p), ("log_sum", C.c_void_p), ("row_state", C.c_void_p),
+                ("n_best", C.c_size_t), ("best_log_prob", C.c_void_p), ("best_index", C.c_void_p)]
+
+
+class AdamWTensor(C.Structure):
+    _fields_ = [("param", C.c_void_p), ("grad", C.c_void_p), ("size", C.c_size_t), ("first", C.c_size_t)]
+
+
+class AdamWArgs(C.Structure):
+    _fields_ = [("param_type", C.c_int), ("grad_type", C.c_int), ("state_bits", C.c_int), ("adam_m", C.c_void_p), ("adam_v", C.c_void_p),
+                ("m_exponent", C.c_void_p), ("v_exponent", C.c_void_p), ("beta_m", C.c_double), ("beta_v", C.c_double),
+                ("epsilon", C.c_double), ("grad_scale", C.c_double), ("decay", C.c_double), ("step_size", C.c_double),
+                ("inv_sqrt_correction", C.c_double), ("key", C.c_uint32), ("schedule", C.c_void_p)]
 
 
 _lib: Optional[C.CDLL] = None
@@ -92,6 +118,21 @@ def load_library() -> C.CDLL:
     lib.kge_microbench_scores.argtypes = [C.c_int, sz, sz, sz, C.c_int, fp]
     lib.kge_op_activation.argtypes = [C.c_int, fp, fp, sz, sz, fp, fp]
     lib.kge_op_all_to_all.argtypes = [fp, sz, sz, fp]
+    ll = C.c_longlong
+    lib.kge_op_log_probs_workspace.argtypes = [sz, sz, sz]
+    lib.kge_op_log_probs_workspace.restype = sz
+    lib.kge_op_log_probs.argtypes = [C.POINTER(Scores), C.POINTER(LogProbsOut), vp, sz, vp]
+    lib.kge_op_log_probs_grad.argtypes = [C.POINTER(Scores), vp, vp, vp, sz, vp, vp, vp, ll, vp]
+    lib.kge_op_rows8_bytes.argtypes = [sz, sz, C.POINTER(sz), C.POINTER(sz)]
+    lib.kge_op_quantise_rows.argtypes = [vp, C.c_int, sz, sz, ll, C.c_int, vp, vp, vp]
+    lib.kge_op_product8_workspace.argtypes = [sz, sz, sz]
+    lib.kge_op_product8_workspace.restype = sz
+    lib.kge_op_product8.argtypes = [vp, vp, sz, vp, vp, sz, sz, vp, C.c_int, ll, vp, sz, vp]
+    lib.kge_op_product8_status.argtypes = []
+    lib.kge_op_adamw.argtypes = [C.POINTER(AdamWArgs), C.POINTER(AdamWTensor), sz, vp]
+    lib.kge_op_adamw_key.argtypes = [C.c_uint32, C.c_uint32]
+    lib.kge_op_adamw_key.restype = C.c_uint32
+    lib.kge_op_adamw_moments.argtypes = [vp, vp, vp, vp, sz, vp, vp, vp]
     _lib = lib
     return lib
 

@@ -6,6 +6,7 @@
 #include <mutex>
 #include <vector>
 
+#include "device_ops.hpp"
 #include "engine.hpp"
 #include "tc_gemm.cuh"
 #include "tc_planes.cuh"
@@ -729,6 +730,65 @@ int kge_op_scatter_add_rows_noalloc(const float* grad_rows, const uint32_t* indi
         k_segment_sum_rows<<<(unsigned)rows, 128, 0, stream>>>(grad_rows, scratch->perm, scratch->offsets, width, grad_table);
         KGE_CUDA(cudaGetLastError());
     });
+}
+
+
+size_t kge_op_log_probs_workspace(size_t rows, size_t cols, size_t n_best) { return log_probs_workspace(rows, cols, n_best); }
+
+int kge_op_log_probs(const kge_scores* scores, const kge_log_probs_out* out, void* workspace, size_t workspace_bytes, void* cuda_stream) {
+    return guarded(g_error, [&] {
+        require(scores && out, "kge_op_log_probs: null argument");
+        log_probs(*scores, *out, workspace, workspace_bytes, static_cast<cudaStream_t>(cuda_stream));
+    });
+}
+
+int kge_op_log_probs_grad(const kge_scores* scores, const float* row_state, const float* grad_log_prob, const float* grad_entropy, size_t n_best,
+                          const int32_t* best_index, const float* grad_best, void* grad_x, long long grad_row_stride, void* cuda_stream) {
+    return guarded(g_error, [&] {
+        require(scores, "kge_op_log_probs_grad: null argument");
+        log_probs_grad(*scores, row_state, grad_log_prob, grad_entropy, n_best, best_index, grad_best, grad_x, grad_row_stride, static_cast<cudaStream_t>(cuda_stream));
+    });
+}
+
+int kge_op_rows8_bytes(size_t rows, size_t cols, size_t* values, size_t* exponents) {
+    return guarded(g_error, [&] {
+        require(values && exponents, "kge_op_rows8_bytes: null argument");
+        rows8_bytes(rows, cols, values, exponents);
+    });
+}
+
+int kge_op_quantise_rows(const void* x, int float_type, size_t rows, size_t cols, long long row_stride, int transposed, uint8_t* values,
+                         uint8_t* exponents, void* cuda_stream) {
+    return guarded(g_error, [&] { quantise_rows(x, float_type, rows, cols, row_stride, transposed != 0, values, exponents, static_cast<cudaStream_t>(cuda_stream)); });
+}
+
+size_t kge_op_product8_workspace(size_t m, size_t n, size_t k) { return product8_workspace(m, n, k); }
+
+int kge_op_product8(const uint8_t* a_values, const uint8_t* a_exponents, size_t m, const uint8_t* b_values, const uint8_t* b_exponents, size_t n,
+                    size_t k, void* out, int out_type, long long out_row_stride, void* workspace, size_t workspace_bytes, void* cuda_stream) {
+    return guarded(g_error, [&] {
+        product8(a_values, a_exponents, m, b_values, b_exponents, n, k, out, out_type, out_row_stride, workspace, workspace_bytes, static_cast<cudaStream_t>(cuda_stream));
+    });
+}
+
+int kge_op_product8_status(void) {
+    return guarded(g_error, [&] {
+        if (product8_gave_up()) fail(KGE_DEVICE_STATUS, "kge_op_product8: a wait on the device gave up");
+    });
+}
+
+int kge_op_adamw(const kge_adamw_args* args, const kge_adamw_tensor* tensors, size_t n_tensors, void* cuda_stream) {
+    return guarded(g_error, [&] {
+        require(args, "kge_op_adamw: null argument");
+        adamw_step(*args, tensors, n_tensors, static_cast<cudaStream_t>(cuda_stream));
+    });
+}
+
+uint32_t kge_op_adamw_key(uint32_t seed, uint32_t step) { return adamw_key(seed, step); }
+
+int kge_op_adamw_moments(const uint8_t* adam_m, const uint8_t* m_exponent, const uint8_t* adam_v, const uint8_t* v_exponent, size_t size, void* m_bf16,
+                         void* v_bf16, void* cuda_stream) {
+    return guarded(g_error, [&] { adamw_moments(adam_m, m_exponent, adam_v, v_exponent, size, m_bf16, v_bf16, static_cast<cudaStream_t>(cuda_stream)); });
 }
 
 }  // extern "C"

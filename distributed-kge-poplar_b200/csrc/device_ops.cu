@@ -1,0 +1,319 @@
+// The operators of a softmax over all candidates on device arrays: checks of their arguments and their launches.
+#include "device_ops.hpp"
+
+#include <cuda.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "adamw.cuh"
+#include "log_probs.cuh"
+#include "rows8.cuh"
+
+namespace kge {
+namespace {
+
+void need(bool ok, const char* what) {
+    if (!ok) fail(KGE_INVALID_ARGUMENT, what);
+}
+bool aligned_to(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+size_t type_bytes(int type, const char* what) {
+    if (type != KGE_F32 && type != KGE_F16 && type != KGE_BF16) fail(KGE_INVALID_ARGUMENT, msg() << what << ": the element type must be KGE_F32, KGE_F16 or KGE_BF16, not " << type);
+    return type == KGE_F32 ? 4 : 2;
+}
+// fn(T()) for the element type named.
+template <class Fn>
+void with_type(int type, Fn&& fn) {
+    if (type == KGE_F32) fn(float());
+    else if (type == KGE_F16) fn(__half());
+    else fn(__nv_bfloat16());
+}
+unsigned grid_of(size_t blocks, const char* what) {
+    if (blocks > 0x7fffffffu) fail(KGE_INVALID_ARGUMENT, msg() << what << ": too large for one launch");
+    return (unsigned)blocks;
+}
+// Allows a kernel its dynamic shared memory, once per device.
+template <auto Kernel>
+void allow_shared_memory(size_t bytes) {
+    static std::atomic<uint64_t> done{0};
+    const int slot = current_device_slot();
+    if (slot >= 0 && (done.load() >> slot & 1)) return;
+    KGE_CUDA(cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    if (slot >= 0) done.fetch_or((uint64_t)1 << slot);
+}
+
+constexpr size_t kMostColumns = 0x7fffffffu - 65536;  // a column and a vector past it fit an int
+
+lp::Scores checked_scores(const kge_scores& s, const char* what) {
+    const size_t bytes = type_bytes(s.float_type, what);
+    if (s.cols > kMostColumns) fail(KGE_INVALID_ARGUMENT, msg() << what << ": " << s.cols << " columns, " << kMostColumns << " are the most");
+    if (s.rows > 1 && s.row_stride < (long long)s.cols) fail(KGE_INVALID_ARGUMENT, msg() << what << ": rows of " << s.cols << " columns, " << s.row_stride << " apart");
+    if (!(s.scale > 0.f) || !std::isfinite(s.scale)) fail(KGE_INVALID_ARGUMENT, msg() << what << ": scale must be positive and finite, not " << s.scale);
+    if (s.rows && s.cols && !s.x) fail(KGE_INVALID_ARGUMENT, msg() << what << ": null scores");
+    if (!aligned_to(s.x, bytes)) fail(KGE_INVALID_ARGUMENT, msg() << what << ": scores are not aligned to their type");
+    if (s.mask && s.mask_stride != 0 && s.rows > 1 && s.mask_stride < (long long)s.cols)
+        fail(KGE_INVALID_ARGUMENT, msg() << what << ": mask rows of " << s.cols << " columns, " << s.mask_stride << " apart");
+    return lp::Scores{s.x, s.mask, s.count, s.target, s.row_stride, s.mask_stride, (int)s.cols, s.scale * lp::kLog2e, s.scale};
+}
+
+}  // namespace
+
+// ---------------------------------------------------------------------------
+
+size_t log_probs_workspace(size_t, size_t, size_t) { return 0; }
+
+void log_probs(const kge_scores& scores, const kge_log_probs_out& out, void*, size_t, cudaStream_t stream) {
+    const char* const what = "kge_op_log_probs";
+    const lp::Scores s = checked_scores(scores, what);
+    if (out.n_best > (size_t)lp::kMaxBest) fail(KGE_INVALID_ARGUMENT, msg() << what << ": n_best is " << out.n_best << ", " << lp::kMaxBest << " is the most");
+    if (scores.rows == 0) return;
+    need(out.log_prob && out.entropy && out.log_sum && out.row_state && (!out.n_best || (out.best_log_prob && out.best_index)), "kge_op_log_probs: null output");
+    need(aligned_to(out.row_state, 16), "kge_op_log_probs: row_state is not aligned to 16 bytes");
+    const lp::Out o{out.log_prob, out.entropy, out.log_sum, reinterpret_cast<float4*>(out.row_state), out.best_log_prob, out.best_index, (int)out.n_best};
+    with_type(scores.float_type, [&](auto t) { lp::k_log_probs<decltype(t)><<<grid_of(scores.rows, what), lp::kThreads, 0, stream>>>(s, o); });
+    KGE_CUDA(cudaGetLastError());
+}
+
+void log_probs_grad(const kge_scores& scores, const float* row_state, const float* grad_log_prob, const float* grad_entropy, size_t n_best,
+                    const int32_t* best_index, const float* grad_best, void* grad_x, long long grad_row_stride, cudaStream_t stream) {
+    const char* const what = "kge_op_log_probs_grad";
+    const lp::Scores s = checked_scores(scores, what);
+    if (n_best > (size_t)lp::kMaxBest) fail(KGE_INVALID_ARGUMENT, msg() << what << ": n_best is " << n_best << ", " << lp::kMaxBest << " is the most");
+    if (scores.rows == 0 || scores.cols == 0) return;
+    need(row_state && grad_x, "kge_op_log_probs_grad: null argument");
+    need(aligned_to(row_state, 16), "kge_op_log_probs_grad: row_state is not aligned to 16 bytes");
+    need(aligned_to(grad_x, type_bytes(scores.float_type, what)), "kge_op_log_probs_grad: the gradient is not aligned to its type");
+    need(!grad_best || !n_best || best_index, "kge_op_log_probs_grad: alternatives with a gradient but no indices");
+    if (scores.rows > 1 && grad_row_stride < (long long)scores.cols)
+        fail(KGE_INVALID_ARGUMENT, msg() << what << ": gradient rows of " << scores.cols << " columns, " << grad_row_stride << " apart");
+    need(grad_x != scores.x || scores.rows == 1 || grad_row_stride == scores.row_stride, "kge_op_log_probs_grad: a gradient in the scores' place has their row stride");
+    const size_t width = 16 / type_bytes(scores.float_type, what);
+    const size_t per_block = (size_t)lp::kGradThreads * lp::kGradVectors;
+    const size_t blocks = ((scores.cols + 2 * width - 2) / width + per_block - 1) / per_block;  // whatever a row's first vector leaves out
+    const lp::GradArgs g{reinterpret_cast<const float4*>(row_state), grad_log_prob, grad_entropy, best_index, n_best ? grad_best : nullptr,
+                         grad_x, grad_row_stride, (int)n_best, (int)blocks};
+    with_type(scores.float_type, [&](auto t) { lp::k_log_probs_grad<decltype(t)><<<grid_of(scores.rows * blocks, what), lp::kGradThreads, 0, stream>>>(s, g); });
+    KGE_CUDA(cudaGetLastError());
+}
+
+// ---------------------------------------------------------------------------
+
+void rows8_bytes(size_t rows, size_t cols, size_t* values, size_t* exponents) {
+    *values = rows * rows8::value_stride(cols);
+    *exponents = (rows + 127) / 128 * rows8::groups_of(cols) * rows8::kGroupBytes;
+}
+
+void quantise_rows(const void* x, int float_type, size_t rows, size_t cols, long long row_stride, bool transposed, uint8_t* values,
+                   uint8_t* exponents, cudaStream_t stream) {
+    const char* const what = "kge_op_quantise_rows";
+    const size_t bytes = type_bytes(float_type, what);
+    if (rows > 1 && row_stride < (long long)cols) fail(KGE_INVALID_ARGUMENT, msg() << what << ": rows of " << cols << " columns, " << row_stride << " apart");
+    if (rows == 0 || cols == 0) return;
+    need(x && values && exponents, "kge_op_quantise_rows: null argument");
+    need(aligned_to(x, bytes), "kge_op_quantise_rows: x is not aligned to its type");
+    need(aligned_to(values, 16) && aligned_to(exponents, 16), "kge_op_quantise_rows: values and exponents must be aligned to 16 bytes");
+    with_type(float_type, [&](auto t) {
+        using T = decltype(t);
+        const T* const src = static_cast<const T*>(x);
+        if (!transposed) {
+            const size_t groups = rows8::groups_of(cols), units = round_up(rows, 128) * groups;
+            rows8::k_quantise_rows<T><<<grid_of((units + 7) / 8, what), 256, 0, stream>>>(src, rows, cols, row_stride, groups, values, exponents);
+        } else {
+            const size_t groups = rows8::groups_of(rows), tiles = round_up(cols, 128) / rows8::kTurnCols;
+            rows8::k_quantise_columns<T><<<grid_of(tiles * groups * 4, what), 256, 0, stream>>>(src, rows, cols, row_stride, groups, values, exponents);
+        }
+    });
+    KGE_CUDA(cudaGetLastError());
+}
+
+namespace {
+
+struct ProductPlan {
+    int tile_m, m_tiles, n_tiles, blocks, splits;
+};
+ProductPlan product_plan(size_t m, size_t n, size_t k) {
+    ProductPlan p;
+    p.tile_m = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128;
+    p.m_tiles = (int)((m + p.tile_m - 1) / p.tile_m);
+    p.n_tiles = (int)((n + rows8::kTileN - 1) / rows8::kTileN);
+    p.blocks = (int)rows8::blocks_of(k);
+    const long long tiles = (long long)p.m_tiles * p.n_tiles;
+    p.splits = (int)std::max<long long>(1, std::min<long long>(tiles ? kSmCount / tiles : 1, p.blocks / 4));
+    return p;
+}
+
+CUtensorMap rows_map(const uint8_t* values, size_t rows, size_t cols, int box_rows) {
+    tc::EncodeTiledFn encode = tc::encode_tiled_fn();
+    if (!encode) fail(KGE_RUNTIME_ERROR, "kge_op_product8: the driver has no cuTensorMapEncodeTiled");
+    CUtensorMap map;
+    const cuuint64_t dims[2] = {cols, rows}, strides[1] = {rows8::value_stride(cols)};
+    const cuuint32_t box[2] = {rows8::kBlock, (cuuint32_t)box_rows}, step[2] = {1, 1};
+    if (encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(values), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+        fail(KGE_RUNTIME_ERROR, "kge_op_product8: a tensor map was refused");
+    return map;
+}
+
+template <int TM, class TOut>
+void launch_product(const CUtensorMap& a, const CUtensorMap& b, const rows8::ProductArgs& g, cudaStream_t stream) {
+    constexpr size_t smem = rows8::Tile<TM>::smem();
+    allow_shared_memory<rows8::k_product8<TM, TOut>>(smem);
+    const int work = g.n_tiles * g.m_tiles * g.splits;
+    rows8::k_product8<TM, TOut><<<std::min(work, kSmCount), rows8::kProductThreads, smem, stream>>>(a, b, g);
+}
+template <class TOut>
+void launch_product(int tile_m, const CUtensorMap& a, const CUtensorMap& b, const rows8::ProductArgs& g, cudaStream_t stream) {
+    if (tile_m == 16) launch_product<16, TOut>(a, b, g, stream);
+    else if (tile_m == 32) launch_product<32, TOut>(a, b, g, stream);
+    else if (tile_m == 64) launch_product<64, TOut>(a, b, g, stream);
+    else launch_product<128, TOut>(a, b, g, stream);
+}
+
+}  // namespace
+
+size_t product8_workspace(size_t m, size_t n, size_t k) {
+    if (m == 0 || n == 0 || k == 0 || m > 0x7fffffffu || n > 0x7fffffffu) return 0;
+    const ProductPlan p = product_plan(m, n, k);
+    return p.splits > 1 ? (size_t)p.splits * m * n * sizeof(float) : 0;
+}
+
+void product8(const uint8_t* a_values, const uint8_t* a_exponents, size_t m, const uint8_t* b_values, const uint8_t* b_exponents, size_t n,
+              size_t k, void* out, int out_type, long long out_row_stride, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
+    const char* const what = "kge_op_product8";
+    const size_t bytes = type_bytes(out_type, what);
+    if (m > 0x7fffffffu || n > 0x7fffffffu - 65536 || k > 0x7fffffffu - 65536) fail(KGE_INVALID_ARGUMENT, msg() << what << ": " << m << " x " << n << " x " << k << " is too large");
+    if (m > 1 && out_row_stride < (long long)n) fail(KGE_INVALID_ARGUMENT, msg() << what << ": rows of " << n << " results, " << out_row_stride << " apart");
+    if (m == 0 || n == 0) return;
+    need(out, "kge_op_product8: null output");
+    need(aligned_to(out, bytes), "kge_op_product8: the output is not aligned to its type");
+    if (k == 0) {
+        KGE_CUDA(cudaMemset2DAsync(out, (size_t)std::max<long long>(out_row_stride, (long long)n) * bytes, 0, n * bytes, m, stream));
+        return;
+    }
+    need(a_values && a_exponents && b_values && b_exponents, "kge_op_product8: null operand");
+    need(aligned_to(a_values, 16) && aligned_to(a_exponents, 16) && aligned_to(b_values, 16) && aligned_to(b_exponents, 16),
+         "kge_op_product8: operands must be aligned to 16 bytes");
+    const ProductPlan p = product_plan(m, n, k);
+    if ((long long)p.m_tiles * p.n_tiles * p.splits > 0x7fffffff) fail(KGE_INVALID_ARGUMENT, msg() << what << ": " << m << " x " << n << " is too large");
+    const size_t wanted = product8_workspace(m, n, k);
+    if (wanted) {
+        if (workspace_bytes < wanted || !workspace) fail(KGE_INVALID_ARGUMENT, msg() << what << ": a workspace of " << wanted << " bytes is wanted, not " << workspace_bytes);
+        need(aligned_to(workspace, 256), "kge_op_product8: the workspace is not aligned to 256 bytes");
+    }
+    const CUtensorMap a = rows_map(a_values, m, k, p.tile_m), b = rows_map(b_values, n, k, rows8::kTileN);
+    rows8::ProductArgs g{a_exponents, b_exponents, out, out_row_stride, 0, (int)m, (int)n, p.blocks, (p.blocks + 3) / 4, p.n_tiles, p.m_tiles, p.splits};
+    if (p.splits > 1) {
+        g.out = workspace;
+        g.out_stride = (long long)n;
+        g.split_stride = (long long)m * (long long)n;
+        launch_product<float>(p.tile_m, a, b, g, stream);
+        with_type(out_type, [&](auto t) {
+            using T = decltype(t);
+            rows8::k_add_splits<T><<<grid_of((m * n + 255) / 256, what), 256, 0, stream>>>(static_cast<const float*>(workspace), g.split_stride, p.splits, (int)m, (int)n,
+                                                                                   static_cast<T*>(out), out_row_stride);
+        });
+    } else {
+        with_type(out_type, [&](auto t) { launch_product<decltype(t)>(p.tile_m, a, b, g, stream); });
+    }
+    KGE_CUDA(cudaGetLastError());
+}
+
+bool product8_gave_up() {
+    unsigned status = 0;
+    KGE_CUDA(cudaMemcpyFromSymbol(&status, rows8::g_product8_status, sizeof status));
+    if (status) {
+        const unsigned zero = 0;
+        KGE_CUDA(cudaMemcpyToSymbol(rows8::g_product8_status, &zero, sizeof zero));
+    }
+    return status != 0;
+}
+
+// ---------------------------------------------------------------------------
+
+namespace {
+
+template <class TP, class TG, int BITS, int MAX>
+void launch_adamw(const adamw::Table<adamw::kMaxTensors>& all, const adamw::Params& p, const kge_adamw_args& a, cudaStream_t stream) {
+    adamw::Table<MAX> table;
+    table.n = all.n;
+    std::copy(all.t, all.t + all.n, table.t);
+    const uint32_t blocks = all.t[all.n - 1].blocks_end;
+    constexpr uint32_t per = adamw::kThreads / 32;
+    adamw::k_adamw<TP, TG, BITS, MAX><<<(blocks + per - 1) / per, adamw::kThreads, 0, stream>>>(table, p, a.adam_m, a.adam_v, a.m_exponent, a.v_exponent);
+    KGE_CUDA(cudaGetLastError());
+}
+template <class TP, class TG, int BITS>
+void launch_adamw(const adamw::Table<adamw::kMaxTensors>& all, const adamw::Params& p, const kge_adamw_args& a, cudaStream_t stream) {
+    if (all.n <= 16) launch_adamw<TP, TG, BITS, 16>(all, p, a, stream);
+    else launch_adamw<TP, TG, BITS, adamw::kMaxTensors>(all, p, a, stream);
+}
+
+}  // namespace
+
+void adamw_step(const kge_adamw_args& a, const kge_adamw_tensor* tensors, size_t n_tensors, cudaStream_t stream) {
+    const char* const what = "kge_op_adamw";
+    if (a.param_type != KGE_F32 && a.param_type != KGE_BF16) fail(KGE_INVALID_ARGUMENT, msg() << what << ": parameters must be KGE_F32 or KGE_BF16, not " << a.param_type);
+    const size_t param_bytes = a.param_type == KGE_F32 ? 4 : 2, grad_bytes = type_bytes(a.grad_type, what);
+    if (a.state_bits != 8 && a.state_bits != 32) fail(KGE_INVALID_ARGUMENT, msg() << what << ": state_bits must be 8 or 32, not " << a.state_bits);
+    need(n_tensors == 0 || tensors, "kge_op_adamw: null tensors");
+    const adamw::Params p{(float)a.beta_m, (float)(1. - a.beta_m), (float)a.beta_v, (float)(1. - a.beta_v), (float)a.epsilon, (float)a.grad_scale,
+                          (float)a.decay, (float)a.step_size, (float)a.inv_sqrt_correction, a.key, a.schedule};
+    adamw::Table<adamw::kMaxTensors> table;
+    table.n = 0;
+    uint32_t blocks = 0;
+    for (size_t i = 0; i < n_tensors; ++i) {
+        const kge_adamw_tensor& t = tensors[i];
+        if (!t.size) continue;
+        if (!t.param || !t.grad) fail(KGE_INVALID_ARGUMENT, msg() << what << ": tensor " << i << " has no parameter or no gradient");
+        if (!aligned_to(t.param, param_bytes) || !aligned_to(t.grad, grad_bytes)) fail(KGE_INVALID_ARGUMENT, msg() << what << ": tensor " << i << " is not aligned to its type");
+        if (t.first % adamw::kBlock) fail(KGE_INVALID_ARGUMENT, msg() << what << ": the moments of tensor " << i << " begin at " << t.first << ", no multiple of " << adamw::kBlock);
+        if ((t.size + adamw::kBlock - 1) / adamw::kBlock > 0x7fffffffu) fail(KGE_INVALID_ARGUMENT, msg() << what << ": tensor " << i << " has " << t.size << " values, too many");
+    }
+    bool any = false;
+    for (size_t i = 0; i < n_tensors; ++i) any = any || tensors[i].size;
+    if (!any) return;
+    need(a.adam_m && a.adam_v && (a.state_bits == 32 || (a.m_exponent && a.v_exponent)), "kge_op_adamw: null moments");
+    need(aligned_to(a.adam_m, 16) && aligned_to(a.adam_v, 16), "kge_op_adamw: the moments are not aligned to 16 bytes");
+    need(!a.schedule || aligned_to(a.schedule, 4), "kge_op_adamw: the schedule is not aligned");
+    const auto flush = [&] {
+        if (table.n == 0) return;
+        with_type(a.grad_type, [&](auto g) {
+            using TG = decltype(g);
+            if (a.param_type == KGE_F32) {
+                if (a.state_bits == 32) launch_adamw<float, TG, 32>(table, p, a, stream);
+                else launch_adamw<float, TG, 8>(table, p, a, stream);
+            } else {
+                if (a.state_bits == 32) launch_adamw<__nv_bfloat16, TG, 32>(table, p, a, stream);
+                else launch_adamw<__nv_bfloat16, TG, 8>(table, p, a, stream);
+            }
+        });
+        table.n = 0;
+        blocks = 0;
+    };
+    for (size_t i = 0; i < n_tensors; ++i) {
+        const kge_adamw_tensor& t = tensors[i];
+        if (!t.size) continue;
+        const uint32_t more = (uint32_t)((t.size + adamw::kBlock - 1) / adamw::kBlock);
+        if (table.n == adamw::kMaxTensors || more > 0x7fffffffu - blocks) flush();
+        blocks += more;
+        table.t[table.n++] = adamw::Tensor{t.param, t.grad, t.size, t.first / adamw::kBlock, blocks, aligned_to(t.param, 4 * param_bytes) && aligned_to(t.grad, 4 * grad_bytes)};
+    }
+    flush();
+}
+
+uint32_t adamw_key(uint32_t seed, uint32_t step) { return adamw::mix(seed * 0x9E3779B9u + step * 0xBB67AE85u); }
+
+void adamw_moments(const uint8_t* adam_m, const uint8_t* m_exponent, const uint8_t* adam_v, const uint8_t* v_exponent, size_t size, void* m_bf16,
+                   void* v_bf16, cudaStream_t stream) {
+    const char* const what = "kge_op_adamw_moments";
+    if (size % adamw::kBlock) fail(KGE_INVALID_ARGUMENT, msg() << what << ": the size is " << size << ", no multiple of " << adamw::kBlock);
+    if (size == 0) return;
+    need(adam_m && m_exponent && adam_v && v_exponent && m_bf16 && v_bf16, "kge_op_adamw_moments: null argument");
+    need(aligned_to(adam_m, 16) && aligned_to(adam_v, 16) && aligned_to(m_bf16, 16) && aligned_to(v_bf16, 16), "kge_op_adamw_moments: moments must be aligned to 16 bytes");
+    const size_t blocks = size / adamw::kBlock, per = adamw::kThreads / 32;
+    adamw::k_moments<<<grid_of((blocks + per - 1) / per, what), adamw::kThreads, 0, stream>>>(adam_m, m_exponent, adam_v, v_exponent, blocks,
+                                                                                            static_cast<__nv_bfloat16*>(m_bf16), static_cast<__nv_bfloat16*>(v_bf16));
+    KGE_CUDA(cudaGetLastError());
+}
+
+}  // namespace kge

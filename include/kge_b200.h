@@ -267,6 +267,137 @@ int kge_op_activation(int kind, const float* x, const float* grad_out, size_t ro
  * blocks of `block` floats (src/pag/pag.cpp:915-935). */
 int kge_op_all_to_all(const float* in, size_t n_shard, size_t block, float* out);
 
+/*
+ * Operators of a softmax over all candidates, on DEVICE arrays.  They have no counterpart in the reference, whose softmax is
+ * over the tails of a batch (src/poplar_kge.cpp:575-600) and whose lists come without probabilities (:812-855).
+ * Common to them:
+ *   - all pointers but the argument structs and their tables are device pointers of the current device; the work is queued on
+ *     `cuda_stream` (a cudaStream_t, or NULL for the default stream) and the call returns without waiting for it.  Nothing is
+ *     allocated and nothing kept between calls, so calls may be captured, and may run at the same time on several streams as
+ *     long as they share no output and no workspace.
+ *   - `workspace` is `workspace_bytes` of device memory, aligned to 256 bytes, whose contents need not be anything before the
+ *     call and are nothing after it; how much is wanted is asked of the ..._workspace function (0: NULL will do).
+ *   - float_type is KGE_F32, KGE_F16 or KGE_BF16; arithmetic is in 32 bits, results are rounded once.
+ *   - sizes of zero are no error: nothing is launched that has nothing to write.
+ */
+enum kge_float_type { KGE_BF16 = 3 }; /* beside KGE_F32 and KGE_F16 */
+
+/*
+ * Scores x [rows, cols] of candidates (contiguous along a row, any row stride of at least cols elements), cols < 2^31 - 2^16.
+ * Column c of row r is live where mask[r * mask_stride + c] is not 0 (mask may be NULL: all; mask_stride may be 0: one mask
+ * for all rows), c < count[r] (count may be NULL) and x is not -infinity.  Logits are scale * x, scale > 0 (it has no gradient).
+ * target[r] is the column asked for; one outside [0, cols) means none (target may be NULL: none anywhere).
+ */
+typedef struct kge_scores {
+    const void* x;
+    int float_type;
+    size_t rows, cols;
+    long long row_stride;
+    const uint8_t* mask;
+    long long mask_stride;
+    const int32_t* count;
+    const int32_t* target;
+    float scale;
+} kge_scores;
+
+/* What kge_op_log_probs writes; every array has one entry (best_*: n_best entries) per row. */
+typedef struct kge_log_probs_out {
+    float* log_prob;       /* of the target: 0 without one, -inf where it is not live */
+    float* entropy;        /* of the distribution over the live columns; 0 where none is live */
+    float* log_sum;        /* log of the sum of exp(logit); -inf where no column is live */
+    float* row_state;      /* [rows, 4], aligned to 16 bytes: what kge_op_log_probs_grad needs of a row */
+    size_t n_best;         /* 0 to 128 */
+    float* best_log_prob;  /* [rows, n_best], highest score first, ties by the lower column; -inf past the live columns */
+    int32_t* best_index;   /* [rows, n_best]; -1 past the live columns */
+} kge_log_probs_out;
+
+/*
+ * Log probability of the target, entropy and the n_best most probable columns of each row, in one pass over the scores.
+ * A live NaN or +infinity makes the row's results NaN, as the formulas do; best_index then holds the columns in the order of
+ * their scores all the same, NaN left out.  Masked places may hold anything.
+ */
+size_t kge_op_log_probs_workspace(size_t rows, size_t cols, size_t n_best);
+int kge_op_log_probs(const kge_scores* scores, const kge_log_probs_out* out, void* workspace, size_t workspace_bytes,
+                     void* cuda_stream);
+/*
+ * The gradient with respect to x of sum_r (grad_log_prob[r] log_prob[r] + grad_entropy[r] entropy[r] + sum_i grad_best[r, i]
+ * best_log_prob[r, i]); each of the three may be NULL (zero).  `scores` is the forward call's, row_state and best_index
+ * [rows, n_best] are what it wrote.  A target or an alternative that is not live, a row without live columns and a column
+ * that is not live have no gradient.  grad_x has the scores' float type and may be x itself (same row stride).
+ */
+int kge_op_log_probs_grad(const kge_scores* scores, const float* row_state, const float* grad_log_prob,
+                          const float* grad_entropy, size_t n_best, const int32_t* best_index, const float* grad_best,
+                          void* grad_x, long long grad_row_stride, void* cuda_stream);
+
+/*
+ * Rows in 8-bit floating point.  Each block of 128 consecutive values of a row (the last one of a row may be shorter) has a
+ * power of two 2^e, the smallest with e >= -127 that brings the block's largest finite value down to 448 (e = 0 for a block
+ * of zeros), and is held as value * 2^-e rounded to 4 exponent and 3 significand bits (e4m3, to nearest, ties to even).  A
+ * power of two costs such a format nothing but half an octave of its range, and the tensor core applies it as it multiplies.
+ * NaN and infinities are held as NaN.
+ *   values     [rows, ld] bytes, ld = cols rounded up to 16 (bytes past cols are 0); aligned to 16 bytes
+ *   exponents  e + 127 in the order in which the tensor core takes them: 512 bytes for each group of 128 rows and 4 blocks, in
+ *              them byte (r % 32) * 16 + (r / 32) * 4 + block % 4 of the group's row r; groups of a row side by side; aligned
+ *              to 16 bytes.  Bytes of rows and blocks that do not exist are 127.
+ * kge_op_rows8_bytes gives the sizes of both.  x [rows, cols] has any row stride of at least cols elements; with `transposed`
+ * the rows that are made are the columns of x: values [cols, ld] with ld = rows rounded up to 16, blocks along a column.
+ */
+int kge_op_rows8_bytes(size_t rows, size_t cols, size_t* values, size_t* exponents);
+int kge_op_quantise_rows(const void* x, int float_type, size_t rows, size_t cols, long long row_stride, int transposed,
+                         uint8_t* values, uint8_t* exponents, void* cuda_stream);
+/*
+ * out[i, j] = sum_c a[i, c] * b[j, c] for two arrays of such rows, a [m, k] and b [n, k]; out [m, n] of out_type with a row
+ * stride of at least n elements.  Products and sums are in 32 bits.  The gradients of the product are products of the same kind:
+ * of grad_out's rows and b's columns, and of the columns of grad_out and a.
+ */
+size_t kge_op_product8_workspace(size_t m, size_t n, size_t k);
+int kge_op_product8(const uint8_t* a_values, const uint8_t* a_exponents, size_t m, const uint8_t* b_values,
+                    const uint8_t* b_exponents, size_t n, size_t k, void* out, int out_type, long long out_row_stride,
+                    void* workspace, size_t workspace_bytes, void* cuda_stream);
+/* KGE_DEVICE_STATUS if a bounded wait inside a kge_op_product8 on the current device has given up since the last question (its
+ * results are not to be used); waits for the device. */
+int kge_op_product8_status(void);
+
+/*
+ * One AdamW step over many tensors at once (the engine's own step for the dense parameters is src/fructose/frnn.cpp:61-90):
+ *   m = beta_m m + (1 - beta_m) g;  v = beta_v v + (1 - beta_v) g^2  with g = grad_scale * grad
+ *   p = p * decay - step_size * m / (sqrt(v) * inv_sqrt_correction + epsilon)
+ * where decay = 1 - learning_rate * weight_decay, step_size = learning_rate / (1 - beta_m^t) and inv_sqrt_correction =
+ * (1 - beta_v^t)^-1/2 in step t.  Parameters are fp32, or bf16 rounded stochastically (nearest would lose every step below
+ * 2^-9 of a value); fp32 moments, or 8-bit ones:
+ *   blocks of 128 values of a tensor; one byte E per block, the exponent (as in an fp32) of its largest value after that is
+ *   rounded up to 3 significand bits, at least 16 (m) or 33 (v), 255: some value is not finite, all are read as NaN;
+ *   v: code c stands for the fp32 whose upper 12 bits are 8 E + 7 - 255 + c, 0 for zero; no v > 0 is rounded to zero, so that
+ *   no step is divided by epsilon alone;  m: sign in bit 7, and c of 7 bits for 8 E + 7 - 127 + c, 0 for zero.
+ * Codes are rounded stochastically, since a step moves v by 1 - beta_v of itself, far less than a code's half.  The draws are
+ * 16 bits each of a 32-bit mix of (key, position), position being the value's place in the moments: m takes bits 0-15, v 16-31, bf16 p 8-23.
+ * Tensor i's moments begin at `first` values (a multiple of 128) in adam_m and adam_v, and at first / 128 in the exponents.
+ */
+typedef struct kge_adamw_tensor {
+    void* param;
+    const void* grad;
+    size_t size;
+    size_t first;
+} kge_adamw_tensor;
+typedef struct kge_adamw_args {
+    int param_type;       /* KGE_F32 or KGE_BF16, of all tensors */
+    int grad_type;        /* KGE_F32, KGE_F16 or KGE_BF16, of all tensors */
+    int state_bits;       /* 8 or 32 */
+    void *adam_m, *adam_v;            /* fp32 or bytes; aligned to 16 bytes */
+    uint8_t *m_exponent, *v_exponent; /* 8 bits only */
+    double beta_m, beta_v, epsilon, grad_scale; /* 1 - beta is taken before anything is rounded to fp32 */
+    double decay, step_size, inv_sqrt_correction;
+    uint32_t key;
+    const float* schedule; /* not NULL: decay, step_size, inv_sqrt_correction and the key's bits are read from these four words on
+                              the device when the kernel runs, for steps captured into a graph and replayed */
+} kge_adamw_args;
+int kge_op_adamw(const kge_adamw_args* args, const kge_adamw_tensor* tensors, size_t n_tensors, void* cuda_stream);
+/* The key of step `step`: what the draws of a seed are mixed with. */
+uint32_t kge_op_adamw_key(uint32_t seed, uint32_t step);
+/* The values that 8-bit moments stand for, as bf16 (exactly); size is a multiple of 128. */
+int kge_op_adamw_moments(const uint8_t* adam_m, const uint8_t* m_exponent, const uint8_t* adam_v, const uint8_t* v_exponent,
+                         size_t size, void* m_bf16, void* v_bf16, void* cuda_stream);
+
 #ifdef __cplusplus
 }
 #endif
