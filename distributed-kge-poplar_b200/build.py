@@ -5,6 +5,7 @@
 Produces, next to this file:
   libkge_b200.so              the C ABI of include/kge_b200.h (CUDA runtime only)
   libpoplar_kge<ext-suffix>   the pybind11 module with the reference's `Engine` class
+  libkge_torch<ext-suffix>    the operators on device arrays for torch tensors (the only part that knows torch)
 A target is rebuilt when any source or header is newer than it.
 """
 
@@ -27,6 +28,7 @@ ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 LIB = HERE / "libkge_b200.so"
 MODULE = HERE / ("libpoplar_kge" + sysconfig.get_config_var("EXT_SUFFIX"))
+TORCH_MODULE = HERE / ("libkge_torch" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 
 def _newer_than(target: Path, sources) -> bool:
@@ -69,6 +71,20 @@ def build(force: bool = False, verbose: bool = False) -> None:
                 os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-Wall",
                 f"-I{pybind11.get_include()}", f"-I{sysconfig.get_paths()['include']}", f"-I{INCLUDE}",
                 binding, "-o", MODULE, f"-L{HERE}", "-lkge_b200", "-Wl,-rpath,$ORIGIN",
+            ],
+            verbose,
+        )
+    binding = CSRC / "torch_binding.cpp"
+    if force or _newer_than(TORCH_MODULE, [binding, INCLUDE / "kge_b200.h"]):
+        from torch.utils import cpp_extension
+
+        includes = [f"-I{p}" for p in cpp_extension.include_paths("cuda") + [sysconfig.get_paths()["include"], INCLUDE]]
+        torch_libs = [f"-L{p}" for p in cpp_extension.library_paths()]
+        _run(
+            [
+                os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-Wall", "-DTORCH_EXTENSION_NAME=libkge_torch", *includes,
+                binding, "-o", TORCH_MODULE, f"-L{HERE}", "-lkge_b200", *torch_libs, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10",
+                "-lc10_cuda", "-Wl,-rpath,$ORIGIN",
             ],
             verbose,
         )
