@@ -60,18 +60,58 @@ lp::Scores checked_scores(const kge_scores& s, const char* what) {
 
 // ---------------------------------------------------------------------------
 
-size_t log_probs_workspace(size_t, size_t, size_t) { return 0; }
+namespace {
 
-void log_probs(const kge_scores& scores, const kge_log_probs_out& out, void*, size_t, cudaStream_t stream) {
+// A row is one block's unless there are too few rows for the GPU's 148 SMs with four blocks each, or its groups of vectors do not
+// fit the block's shared memory.
+struct LogProbsPlan {
+    int threads, parts, vectors;
+    size_t sums_bytes, bytes;
+};
+LogProbsPlan log_probs_plan(size_t rows, size_t cols, size_t n_best, size_t width) {
+    LogProbsPlan p;
+    const size_t all = (cols + 2 * width - 2) / width;  // whatever a row's first vector leaves out
+    p.threads = all <= 512 ? 128 : 256;
+    const size_t most = (size_t)p.threads * lp::kGroupsPerThread<256> * lp::kGroup, least = 1024, wanted = (n_best ? 2 : 4) * kSmCount;
+    size_t parts = std::min(wanted / std::max<size_t>(1, rows), all / least);
+    parts = std::max<size_t>(1, std::max(parts, (all + most - 1) / most));
+    p.vectors = (int)std::max<size_t>(1, (all + parts - 1) / parts);
+    p.parts = (int)std::max<size_t>(1, (all + p.vectors - 1) / p.vectors);
+    p.sums_bytes = round_up(rows * (size_t)p.parts * sizeof(float4), 256);
+    p.bytes = p.parts > 1 ? p.sums_bytes + rows * (size_t)p.parts * n_best * sizeof(unsigned long long) : 0;
+    return p;
+}
+
+}  // namespace
+
+size_t log_probs_workspace(size_t rows, size_t cols, size_t n_best) {
+    if (rows == 0 || cols > kMostColumns || n_best > (size_t)lp::kMaxBest) return 0;
+    return std::max(log_probs_plan(rows, cols, n_best, 4).bytes, log_probs_plan(rows, cols, n_best, 8).bytes);
+}
+
+void log_probs(const kge_scores& scores, const kge_log_probs_out& out, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
     const char* const what = "kge_op_log_probs";
     const lp::Scores s = checked_scores(scores, what);
     if (out.n_best > (size_t)lp::kMaxBest) fail(KGE_INVALID_ARGUMENT, msg() << what << ": n_best is " << out.n_best << ", " << lp::kMaxBest << " is the most");
     if (scores.rows == 0) return;
     need(out.log_prob && out.entropy && out.log_sum && out.row_state && (!out.n_best || (out.best_log_prob && out.best_index)), "kge_op_log_probs: null output");
     need(aligned_to(out.row_state, 16), "kge_op_log_probs: row_state is not aligned to 16 bytes");
+    const size_t wanted = log_probs_workspace(scores.rows, scores.cols, out.n_best);
+    if (wanted) {
+        if (workspace_bytes < wanted || !workspace) fail(KGE_INVALID_ARGUMENT, msg() << what << ": a workspace of " << wanted << " bytes is wanted, not " << workspace_bytes);
+        need(aligned_to(workspace, 256), "kge_op_log_probs: the workspace is not aligned to 256 bytes");
+    }
+    const LogProbsPlan p = log_probs_plan(scores.rows, scores.cols, out.n_best, 16 / type_bytes(scores.float_type, what));
     const lp::Out o{out.log_prob, out.entropy, out.log_sum, reinterpret_cast<float4*>(out.row_state), out.best_log_prob, out.best_index, (int)out.n_best};
-    with_type(scores.float_type, [&](auto t) { lp::k_log_probs<decltype(t)><<<grid_of(scores.rows, what), lp::kThreads, 0, stream>>>(s, o); });
-    KGE_CUDA(cudaGetLastError());
+    const lp::Parts parts{p.parts, p.vectors, static_cast<float4*>(workspace),
+                          reinterpret_cast<unsigned long long*>(static_cast<char*>(workspace) + (workspace ? p.sums_bytes : 0))};
+    const unsigned blocks = grid_of(scores.rows * (size_t)p.parts, what);
+    with_type(scores.float_type, [&](auto t) {
+        using T = decltype(t);
+        if (p.threads == 128) KGE_CUDA(launch_dependent(lp::k_log_probs<T, 128>, dim3(blocks), dim3(128), 0, stream, s, o, parts));
+        else KGE_CUDA(launch_dependent(lp::k_log_probs<T, 256>, dim3(blocks), dim3(256), 0, stream, s, o, parts));
+        if (p.parts > 1) KGE_CUDA(launch_dependent(lp::k_join_parts<T>, dim3((unsigned)scores.rows), dim3(lp::kJoinThreads), 0, stream, s, o, parts));
+    });
 }
 
 void log_probs_grad(const kge_scores& scores, const float* row_state, const float* grad_log_prob, const float* grad_entropy, size_t n_best,
@@ -88,12 +128,12 @@ void log_probs_grad(const kge_scores& scores, const float* row_state, const floa
         fail(KGE_INVALID_ARGUMENT, msg() << what << ": gradient rows of " << scores.cols << " columns, " << grad_row_stride << " apart");
     need(grad_x != scores.x || scores.rows == 1 || grad_row_stride == scores.row_stride, "kge_op_log_probs_grad: a gradient in the scores' place has their row stride");
     const size_t width = 16 / type_bytes(scores.float_type, what);
-    const size_t per_block = (size_t)lp::kGradThreads * lp::kGradVectors;
+    const size_t per_block = (size_t)lp::kGradThreads * lp::kGroup;
     const size_t blocks = ((scores.cols + 2 * width - 2) / width + per_block - 1) / per_block;  // whatever a row's first vector leaves out
     const lp::GradArgs g{reinterpret_cast<const float4*>(row_state), grad_log_prob, grad_entropy, best_index, n_best ? grad_best : nullptr,
-                         grad_x, grad_row_stride, (int)n_best, (int)blocks};
-    with_type(scores.float_type, [&](auto t) { lp::k_log_probs_grad<decltype(t)><<<grid_of(scores.rows * blocks, what), lp::kGradThreads, 0, stream>>>(s, g); });
-    KGE_CUDA(cudaGetLastError());
+                         grad_x, grad_row_stride, (int)n_best, (int)blocks, (uint32_t)scores.rows};
+    const unsigned grid = grid_of(scores.rows * blocks, what);
+    with_type(scores.float_type, [&](auto t) { KGE_CUDA(launch_dependent(lp::k_log_probs_grad<decltype(t)>, dim3(grid), dim3(lp::kGradThreads), 0, stream, s, g)); });
 }
 
 // ---------------------------------------------------------------------------
@@ -159,7 +199,7 @@ void launch_product(const CUtensorMap& a, const CUtensorMap& b, const rows8::Pro
     constexpr size_t smem = rows8::Tile<TM>::smem();
     allow_shared_memory<rows8::k_product8<TM, TOut>>(smem);
     const int work = g.n_tiles * g.m_tiles * g.splits;
-    rows8::k_product8<TM, TOut><<<std::min(work, kSmCount), rows8::kProductThreads, smem, stream>>>(a, b, g);
+    rows8::k_product8<TM, TOut><<<std::min(work, kSmCount), rows8::Tile<TM>::kThreads, smem, stream>>>(a, b, g);
 }
 template <class TOut>
 void launch_product(int tile_m, const CUtensorMap& a, const CUtensorMap& b, const rows8::ProductArgs& g, cudaStream_t stream) {

@@ -77,7 +77,8 @@ static __global__ void __launch_bounds__(256) k_quantise_rows(const T* __restric
 #pragma unroll
         for (int q = 0; q < 16 / V; ++q) {
             float part[V];
-            lp::unpack(reinterpret_cast<const uint4*>(src)[q], part, T());
+            const uint4 t = reinterpret_cast<const uint4*>(src)[q];
+            lp::unpack<T>(lp::Vector{{t.x, t.y, t.z, t.w}}, part);
 #pragma unroll
             for (int j = 0; j < V; ++j) v[q * V + j] = part[j];
         }
@@ -163,11 +164,14 @@ struct ProductArgs {
 // columns), not the other way round: consecutive lanes then hold consecutive columns of `out`, and a warp stores one row's 32
 // of them at once.
 constexpr int kTileN = 128;
-constexpr int kEpilogueWarps = 4;
-constexpr int kProductThreads = 32 * (2 + kEpilogueWarps);
 constexpr int kTmemColumns = 512;
 template <int TM>
 struct Tile {
+    // Four warps reach a tile's 128 lanes; from 64 columns on eight share them, two to a scheduler.
+    static constexpr int kColumnWarps = TM >= 64 ? 2 : 1;
+    static constexpr int kEpilogueWarps = 4 * kColumnWarps;
+    static constexpr int kThreads = 32 * (2 + kEpilogueWarps);
+    static constexpr int kWarpColumns = TM / kColumnWarps;
     static constexpr int kAGroups = (TM + 127) / 128;
     static constexpr int kBBytes = kTileN * kBlock, kABytes = TM * kBlock;
     static constexpr int kStageBytes = kBBytes + kABytes + kGroupBytes * (1 + kAGroups);
@@ -221,10 +225,32 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile in
     return false;
 }
 
+// One column of the tile per row of `out`.  With a row's address and a test for each store a tile took 5.8 us, a dependent chain
+// of some ten instructions a store with one warp to a scheduler; four addresses apart and no tests leave two.
+template <int ROWS, class TOut>
+__device__ __forceinline__ void store_columns(TOut* out, long long stride, const uint32_t (&acc)[32], int rows) {
+    if (rows == ROWS) {
+        TOut *p0 = out, *p1 = out + stride, *p2 = p1 + stride, *p3 = p2 + stride;
+        const long long four = 4 * stride;
+#pragma unroll
+        for (int j = 0; j < ROWS; j += 4) {
+            lp::store_rounded(p0, __uint_as_float(acc[j]));
+            lp::store_rounded(p1, __uint_as_float(acc[j + 1]));
+            lp::store_rounded(p2, __uint_as_float(acc[j + 2]));
+            lp::store_rounded(p3, __uint_as_float(acc[j + 3]));
+            p0 += four, p1 += four, p2 += four, p3 += four;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < ROWS; ++j)
+            if (j < rows) lp::store_rounded(out + j * stride, __uint_as_float(acc[j]));
+    }
+}
+
 // Warp 0 fetches, warp 1 multiplies, the others write out; a block takes one tile after another, and its next tile is fetched
 // and multiplied while the last one is written.
 template <int TM, class TOut>
-static __global__ void __launch_bounds__(kProductThreads, 1)
+static __global__ void __launch_bounds__(Tile<TM>::kThreads, 1)
 k_product8(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap b_map, ProductArgs g) {
     using L = Tile<TM>;
     extern __shared__ uint8_t smem_raw[];
@@ -236,7 +262,7 @@ k_product8(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CU
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < L::kStages; ++i) tc::mbar_init(&s_full[i], 1), tc::mbar_init(&s_empty[i], 1);
-        for (int i = 0; i < L::kAccumulators; ++i) tc::mbar_init(&s_done[i], 1), tc::mbar_init(&s_free[i], kEpilogueWarps);
+        for (int i = 0; i < L::kAccumulators; ++i) tc::mbar_init(&s_done[i], 1), tc::mbar_init(&s_free[i], L::kEpilogueWarps);
         tc::mbar_fence_init();
         s_gave_up = 0;
     }
@@ -304,21 +330,22 @@ k_product8(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CU
         }
     } else {
         const int quad = warp & 3;  // the lanes that this warp may read
+        const int column0 = (warp - 2) / 4 * L::kWarpColumns;
         int slot = 0;
         uint32_t parity = 0;
         for (int w = blockIdx.x; w < n_work; w += gridDim.x) {
             const int mt = w % g.m_tiles, nt = w / g.m_tiles % g.n_tiles, split = w / (g.m_tiles * g.n_tiles);
             if (!wait(&s_done[slot], parity, gave_up)) break;
             tc::tc_fence_after();
-            const int n = nt * kTileN + quad * 32 + lane, m0 = mt * TM;
-            TOut* const out = static_cast<TOut*>(g.out) + (size_t)split * g.split_stride + n;
+            const int n = nt * kTileN + quad * 32 + lane, m0 = mt * TM + column0;
+            TOut* const out = static_cast<TOut*>(g.out) + (size_t)split * g.split_stride + (long long)m0 * g.out_stride + n;
 #pragma unroll
-            for (int c = 0; c < TM; c += 32) {
+            for (int c = 0; c < L::kWarpColumns; c += 32) {
                 uint32_t acc[32];
-                tc::tmem_ld32(tmem + slot * L::kColumns + c + ((uint32_t)(quad * 32) << 16), acc);
-#pragma unroll
-                for (int j = 0; j < (TM < 32 ? TM : 32); ++j)
-                    if (n < g.n && m0 + c + j < g.m) lp::store_rounded(out + (long long)(m0 + c + j) * g.out_stride, __uint_as_float(acc[j]));
+                tc::tmem_ld32(tmem + slot * L::kColumns + column0 + c + ((uint32_t)(quad * 32) << 16), acc);
+                constexpr int kRows = L::kWarpColumns < 32 ? L::kWarpColumns : 32;
+                const int rows = min(kRows, g.m - m0 - c);
+                store_columns<kRows>(out + (long long)c * g.out_stride, g.out_stride, acc, n < g.n ? rows : 0);
             }
             tc::tc_fence_before();
             __syncwarp();

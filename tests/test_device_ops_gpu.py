@@ -103,6 +103,52 @@ def test_log_probs_of_strided_rows_with_masks_and_counts(ops, dtype):
     check_log_probs(got, forms.log_probs(x, target, one.expand(rows, cols), n_best=3), cols)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,cols,n_best", [(1, 300_007, 128), (3, 150_000, 0), (5, 600_001, 20)])
+def test_log_probs_of_rows_in_parts(ops, rows, cols, n_best, dtype):
+    """Few long rows: each is cut into parts.  Counts end inside a part, at one's start and before all but the first."""
+    g = gen(cols)
+    x = (torch.randn(rows, cols, generator=g) * 3).to(dtype)
+    x[rows - 1, ::2] = 2.0  # equal scores in every part
+    target = torch.randint(cols, (rows,), generator=g, dtype=torch.int32)
+    count = torch.tensor([cols, 70_000, 5, cols // 2, cols - 1][:rows], dtype=torch.int32)
+    for c in (None, count):
+        got = ops.log_probs(x.cuda(), target.cuda(), count=cuda(c), n_best=n_best)
+        check_log_probs(got, forms.log_probs(x, target, count=c, n_best=n_best), cols)
+        again = ops.log_probs(x.cuda(), target.cuda(), count=cuda(c), n_best=n_best)
+        assert torch.equal(got.log_sum, again.log_sum) and torch.equal(got.entropy, again.entropy)
+
+
+def test_log_probs_of_equal_scores_in_many_parts(ops):
+    """More columns than any list of candidates holds share the best score: the lowest columns are listed."""
+    x = torch.zeros(2, 400_000)
+    x[1, 100::7] = 1.0
+    got = ops.log_probs(x.cuda(), n_best=128)
+    assert torch.equal(got.best_index[0].cpu(), torch.arange(128, dtype=torch.int32))
+    assert torch.equal(got.best_index[1].cpu(), torch.arange(128, dtype=torch.int32) * 7 + 100)
+
+
+@pytest.mark.parametrize("scale", [1e-6, 1e-3, 30.0])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_log_probs_of_small_and_large_scales(ops, dtype, scale):
+    """-inf stays out of the sums where a step of the scale reaches from any score to any other."""
+    g = gen(2)
+    x = (torch.randn(4, 3000, generator=g) * 2).to(dtype)
+    x[1, ::2] = -math.inf
+    x[2] = torch.finfo(dtype).min
+    x[2, 5:50] = -math.inf
+    x[3, 7] = torch.finfo(dtype).min
+    want = forms.log_probs(x, torch.full((4,), 2, dtype=torch.int32), scale=scale, n_best=5)
+    got = ops.log_probs(x.cuda(), torch.full((4,), 2, dtype=torch.int32).cuda(), scale=scale, n_best=5)
+    assert torch.equal(got.best_index.cpu(), want["best_index"])
+    for name in ("log_prob", "best_log_prob"):
+        g, w = getattr(got, name).cpu().double(), want[name]
+        tol = log_tolerance(3000, w)
+        assert torch.all((g == w) | ((g - w).abs() <= tol)), name
+    g, w = got.entropy.cpu().double(), want["entropy"]
+    assert torch.all((g - w).abs() <= log_tolerance(3000, w) * (1 + w))
+
+
 def test_log_probs_of_special_rows(ops):
     lowest = torch.finfo(torch.float32).min
     cols = 5000
