@@ -62,8 +62,9 @@ lp::Scores checked_scores(const kge_scores& s, const char* what) {
 
 namespace {
 
-// A row is one block's unless there are too few rows for the GPU's 148 SMs with four blocks each, or its groups of vectors do not
-// fit the block's shared memory.
+// A row is one block's, of as many threads as give each SM 1024 (lp_rank: 128 rows of 100 003 bf16 scores with lists of 100 take
+// LPRANK1 us by blocks of 1024 threads and LPRANK4 in parts of 256), unless there are so few rows that they are cut into parts, four to an
+// SM, or a row's groups of vectors do not fit a block's shared memory.
 struct LogProbsPlan {
     int threads, parts, vectors;
     size_t sums_bytes, bytes;
@@ -71,15 +72,36 @@ struct LogProbsPlan {
 LogProbsPlan log_probs_plan(size_t rows, size_t cols, size_t n_best, size_t width) {
     LogProbsPlan p;
     const size_t all = (cols + 2 * width - 2) / width;  // whatever a row's first vector leaves out
-    p.threads = all <= 512 ? 128 : 256;
-    const size_t most = (size_t)p.threads * lp::kGroupsPerThread<256> * lp::kGroup, least = 1024, wanted = (n_best ? 2 : 4) * kSmCount;
-    size_t parts = std::min(wanted / std::max<size_t>(1, rows), all / least);
-    parts = std::max<size_t>(1, std::max(parts, (all + most - 1) / most));
+    const auto most = [](int threads) {
+        const int groups = threads == 1024 ? lp::Lists<1024>::kGroups : threads == 512 ? lp::Lists<512>::kGroups : threads == 256 ? lp::Lists<256>::kGroups : lp::Lists<128>::kGroups;
+        return (size_t)threads * groups * lp::kGroup;
+    };
+    size_t parts = 1;
+    if (all <= 512) {
+        p.threads = 128;
+    } else {
+        p.threads = rows <= kSmCount + 12 ? 1024 : rows <= 2 * kSmCount + 24 ? 512 : 256;
+        while (p.threads > 256 && (size_t)p.threads * 2 > all) p.threads /= 2;  // two vectors a thread at least
+        if (all > most(p.threads) || (rows <= kSmCount / 2 && (all > 16384 || (rows <= 16 && all >= 2048)))) {
+            p.threads = 256;
+            parts = std::max((all + most(256) - 1) / most(256), std::min(4 * kSmCount / std::max<size_t>(1, rows), all / 1024));
+        }
+    }
     p.vectors = (int)std::max<size_t>(1, (all + parts - 1) / parts);
     p.parts = (int)std::max<size_t>(1, (all + p.vectors - 1) / p.vectors);
     p.sums_bytes = round_up(rows * (size_t)p.parts * sizeof(float4), 256);
     p.bytes = p.parts > 1 ? p.sums_bytes + rows * (size_t)p.parts * n_best * sizeof(unsigned long long) : 0;
     return p;
+}
+
+template <class T>
+void launch_log_probs(int threads, unsigned blocks, const lp::Scores& s, const lp::Out& o, const lp::Parts& parts, cudaStream_t stream) {
+    cudaError_t err;
+    if (threads == 128) err = launch_dependent(lp::k_log_probs<T, 128>, dim3(blocks), dim3(128), 0, stream, s, o, parts);
+    else if (threads == 256) err = launch_dependent(lp::k_log_probs<T, 256>, dim3(blocks), dim3(256), 0, stream, s, o, parts);
+    else if (threads == 512) err = launch_dependent(lp::k_log_probs<T, 512>, dim3(blocks), dim3(512), 0, stream, s, o, parts);
+    else err = launch_dependent(lp::k_log_probs<T, 1024>, dim3(blocks), dim3(1024), 0, stream, s, o, parts);
+    KGE_CUDA(err);
 }
 
 }  // namespace
@@ -108,9 +130,15 @@ void log_probs(const kge_scores& scores, const kge_log_probs_out& out, void* wor
     const unsigned blocks = grid_of(scores.rows * (size_t)p.parts, what);
     with_type(scores.float_type, [&](auto t) {
         using T = decltype(t);
-        if (p.threads == 128) KGE_CUDA(launch_dependent(lp::k_log_probs<T, 128>, dim3(blocks), dim3(128), 0, stream, s, o, parts));
-        else KGE_CUDA(launch_dependent(lp::k_log_probs<T, 256>, dim3(blocks), dim3(256), 0, stream, s, o, parts));
-        if (p.parts > 1) KGE_CUDA(launch_dependent(lp::k_join_parts<T>, dim3((unsigned)scores.rows), dim3(lp::kJoinThreads), 0, stream, s, o, parts));
+        launch_log_probs<T>(p.threads, blocks, s, o, parts, stream);
+        // a short join has few lists to look through, a long one is done sooner by more warps
+        if (p.parts > 32 && out.n_best) {
+            const cudaError_t err = launch_dependent(lp::k_join_parts<T, 1024>, dim3((unsigned)scores.rows), dim3(1024), 0, stream, s, o, parts);
+            KGE_CUDA(err);
+        } else if (p.parts > 1) {
+            const cudaError_t err = launch_dependent(lp::k_join_parts<T, 256>, dim3((unsigned)scores.rows), dim3(256), 0, stream, s, o, parts);
+            KGE_CUDA(err);
+        }
     });
 }
 

@@ -46,9 +46,6 @@ struct Out {
 constexpr int kMaxBest = 128;
 constexpr int kCandidates = 1024;   // columns, or groups of columns, that pass the first threshold
 constexpr int kGroup = 4;           // 16-byte vectors that a thread fetches at once
-// Groups of a thread in one part of a row: their largest scores are kept in shared memory.
-template <int THREADS>
-constexpr int kGroupsPerThread = THREADS == 128 ? 1 : 16;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kNoReference = -FLT_MAX;  // no live score is below
 constexpr float kFarBelow = -200.f;  // 2^-200 is 0 in fp32: exponents below give the same terms, and 0 * -inf stays out
@@ -311,17 +308,28 @@ struct Sums {
     }
 };
 __device__ __forceinline__ Sums none_yet() { return Sums{kNoReference, 0.f, 0.f}; }
+// Of each warp in shared memory: the largest scores of its groups of vectors, and, in the same place afterwards, the groups that
+// reach the threshold and the columns that do.  A part of a row has at most THREADS * kGroups groups.
+template <int THREADS>
+struct Lists {
+    static constexpr int kGroups = THREADS == 128 ? 4 : THREADS == 256 ? 16 : THREADS == 512 ? 8 : 5;
+    static constexpr int kHits = THREADS <= 256 ? 96 : THREADS == 512 ? 64 : 32;
+    static constexpr int kKeys = THREADS <= 256 ? 184 : THREADS == 512 ? 96 : 64;
+    static constexpr int kSlots = kHits + 2 * kKeys > 32 * kGroups ? kHits + 2 * kKeys : 32 * kGroups;
+};
+
 template <int THREADS>
 struct Shared {
-    float group_max[THREADS == 128 ? 128 * kGroup : THREADS * kGroupsPerThread<THREADS>];  // later a list of vectors
+    static constexpr int kWarps = THREADS / 32;
+    alignas(16) float groups[kWarps][Lists<THREADS>::kSlots];
     alignas(16) unsigned long long key[kCandidates + 1];
-    int hit[kCandidates];
-    uint16_t bin[THREADS];
+    uint32_t bound[kWarps];
+    int reach[8][kWarps];
+    int rank[THREADS];
     uint32_t histogram[256];
-    float warp_top[THREADS / 32];
-    float2 warp_sums[THREADS / 32];
-    uint32_t threshold;
-    int hits, vectors, count;
+    float warp_top[kWarps];
+    float2 warp_sums[kWarps];
+    int count, overflow;
     unsigned long long prefix;
     int wanted;
 };
@@ -406,54 +414,147 @@ __device__ __noinline__ void select_exactly(const Row<T>& row, int v0, int v1, i
     __syncthreads();
 }
 
-// A threshold that `wanted` of the block's threads' keys reach, if so many are not 0: their wanted-th largest, cut to its upper 16
-// bits (a few more reach that).  One warp finds it bit by bit: 16 counts of the keys that reach a candidate, 12 instructions each,
-// where ranking 256 keys against one another took as many as all sums of a row of 32 000 scores.
+// A threshold that at least `wanted` of the block's threads' keys reach, if so many are not 0 (else 1).  Each warp sorts its lanes'
+// keys; the least of the W warps' ceil(wanted / W)-th ones is reached by enough, and of eight of them the largest that is is taken:
+// within a tenth of `wanted` for scores in no order.  950 cycles for 256 keys; the exact one, found by bits, took one warp 2300.
 template <int THREADS>
 __device__ __forceinline__ uint32_t first_threshold(uint32_t mine, int wanted, Shared<THREADS>& sh) {
-    sh.bin[threadIdx.x] = (uint16_t)(mine >> 16);
-    if (threadIdx.x == 0) sh.hits = sh.vectors = sh.count = 0;
-    __syncthreads();
-    if (threadIdx.x < 32) {
-        constexpr int kPer = THREADS / 32;
-        uint32_t bin[kPer], found = 0;
+    constexpr int kWarps = THREADS / 32;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+    uint32_t sorted = mine;  // largest in lane 0
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) bin[i] = sh.bin[i * 32 + threadIdx.x];
-#pragma unroll 1
-        for (uint32_t bit = 0x8000u; bit; bit >>= 1) {
-            uint32_t reach = 0;
+    for (int size = 2; size <= 32; size <<= 1)
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) reach += bin[i] >= (found | bit);
-            if ((int)__reduce_add_sync(~0u, reach) >= wanted) found |= bit;
+        for (int stride = size >> 1; stride > 0; stride >>= 1) {
+            const uint32_t other = __shfl_xor_sync(~0u, sorted, stride);
+            sorted = ((lane & size) == 0) == ((lane & stride) == 0) ? max(sorted, other) : min(sorted, other);
         }
-        if (threadIdx.x == 0) sh.threshold = max(found << 16, 1u);
+    if (lane == (wanted + kWarps - 1) / kWarps - 1) sh.bound[warp] = sorted;
+    if (threadIdx.x == 0) sh.count = sh.overflow = 0;
+    __syncthreads();
+    constexpr int kBounds = kWarps < 8 ? kWarps : 8;
+    uint32_t bound[kBounds];
+#pragma unroll
+    for (int i = 0; i < kBounds; ++i) {
+        bound[i] = sh.bound[i];
+        const int reach = __popc(__ballot_sync(~0u, mine >= bound[i]));
+        if (lane == i) sh.reach[i][warp] = reach;
     }
     __syncthreads();
-    return sh.threshold;
+    uint32_t threshold = max(1u, __reduce_min_sync(~0u, lane < kWarps ? sh.bound[lane] : ~0u));
+#pragma unroll
+    for (int i = 0; i < kBounds; ++i) {
+        int reach = 0;
+        if (kWarps <= 8) {
+#pragma unroll
+            for (int j = 0; j < kWarps; ++j) reach += sh.reach[i][j];
+        } else {
+            reach = __reduce_add_sync(~0u, lane < kWarps ? sh.reach[i][lane] : 0);
+        }
+        if (reach >= wanted) threshold = max(threshold, bound[i]);
+    }
+    return threshold;
 }
 
-// put(position, key) for the first n_best of the block's candidates in the order of their scores.  Each is compared with all, by
-// several threads where there are more threads than candidates.
+// Adds what the lanes have to a list of the warp's, in order; returns the list's new length, past `most` without the rest.
+template <class V>
+__device__ __forceinline__ int append(V* list, int length, int most, bool mine, V v) {
+    const uint32_t who = __ballot_sync(~0u, mine);
+    const int at = length + __popc(who & ((1u << (threadIdx.x & 31)) - 1u));
+    if (mine && at < most) list[at] = v;
+    return length + __popc(who);
+}
+// Room for `length` more in the block's list of candidates, for all lanes of a warp.
+template <int THREADS>
+__device__ __forceinline__ int reserve(Shared<THREADS>& sh, int length) {
+    int at = 0;
+    if ((threadIdx.x & 31) == 0 && length) at = atomicAdd(&sh.count, length);
+    return __shfl_sync(~0u, at, 0);
+}
+
+// The columns of the part [v0, v1) that reach the threshold, as the block's candidates.  Each warp looks through its own groups, of
+// those that reach it through the vectors and their columns, its lanes sharing the groups' vectors out anew.  (Lists of the block's
+// with one counter for all took 2000 cycles of additions to it for 130 groups.)
+template <int THREADS, class T>
+__device__ __forceinline__ void collect(const Row<T>& row, int v0, int v1, uint32_t threshold, Shared<THREADS>& sh) {
+    using W = Words<T>;
+    constexpr int V = Row<T>::V;
+    const int lane = threadIdx.x & 31;
+    float* const groups = sh.groups[threadIdx.x / 32];
+    int* const hit = reinterpret_cast<int*>(groups);  // never longer than the groups that have been looked at
+    constexpr int kWarpHits = Lists<THREADS>::kHits, kWarpKeys = Lists<THREADS>::kKeys;
+    unsigned long long* const list = reinterpret_cast<unsigned long long*>(groups + kWarpHits);
+    int hits = 0, at = 0, length = 0;
+    for (int base = v0 + ((int)threadIdx.x & ~31); base < v1; base += THREADS * kGroup, at += 32) {  // the warp's first vector
+        const float top = groups[at + lane];
+        __syncwarp();
+        hits = append(hit, hits, kWarpHits, base + lane < v1 && order_key(top) >= threshold, base + lane);
+    }
+    __syncwarp();
+    for (int i = lane; i - lane < min(hits, kWarpHits) * kGroup; i += 64) {
+        Vector raw[2];
+        int v[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {  // two in flight
+            v[u] = i + 32 * u < min(hits, kWarpHits) * kGroup ? hit[(i + 32 * u) / kGroup] + i % kGroup * THREADS : v1;
+            raw[u] = v[u] < v1 ? row.load(v[u]) : Row<T>::none();
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const uint32_t top = W::larger(W::larger(raw[u].w[0], raw[u].w[1]), W::larger(raw[u].w[2], raw[u].w[3]));
+            if (!__any_sync(~0u, order_key(W::largest(top)) >= threshold)) continue;
+            float val[V];
+            unpack<T>(raw[u], val);
+            const int c0 = row.first_column(v[u]);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const uint32_t key = order_key(val[j]);
+                length = append(list, length, kWarpKeys, key >= threshold, candidate(key, c0 + j));
+            }
+        }
+    }
+    __syncwarp();
+    if (hits > kWarpHits || length > kWarpKeys) {
+        if (lane == 0) sh.overflow = 1;
+        return;
+    }
+    const int room = reserve(sh, length);
+    for (int i = lane; i < length; i += 32)
+        if (room + i < kCandidates) sh.key[room + i] = list[i];
+}
+
+// put(position, key) for the first n_best of the block's candidates in the order of their scores.  Each is compared with all, which
+// all lanes read two at a time, by as many warps' threads as there are, a share each.  (131 of 256 threads' keys: 1960 cycles; a
+// sort of 256 took 2330, lanes sharing a key 3800.)
 template <int THREADS, class Put>
 __device__ __forceinline__ void rank_candidates(int n_best, Shared<THREADS>& sh, Put&& put) {
-    const int n = min(sh.count, kCandidates);
+    const int n = min(sh.count, kCandidates), pairs = (n + 1) / 2;
+    sh.rank[threadIdx.x] = 0;
     if ((n & 1) && threadIdx.x == 0) sh.key[n] = 0;
     __syncthreads();
     const ulonglong2* const keys = reinterpret_cast<const ulonglong2*>(sh.key);
-    const int pairs = (n + 1) / 2;
-    const int share = n <= THREADS / 4 ? 4 : n <= THREADS / 2 ? 2 : 1;  // threads to a candidate, lanes side by side
-    const int from = (int)threadIdx.x % share, step = share;
-    for (int base = 0; base < n; base += THREADS / share) {
-        const int i = base + (int)threadIdx.x / share;
-        const unsigned long long key = i < n ? sh.key[i] : ~0ull;
+    const auto above = [&](unsigned long long key, int from, int to) {
         int rank = 0;
-#pragma unroll 4
-        for (int j = from; j < pairs; j += step) {
+#pragma unroll 8
+        for (int j = from; j < to; ++j) {
             const ulonglong2 two = keys[j];
             rank += (two.x > key) + (two.y > key);
         }
-        for (int o = 1; o < share; o <<= 1) rank += __shfl_xor_sync(~0u, rank, o);
-        if (i < n && from == 0 && rank < n_best) put(rank, key);
+        return rank;
+    };
+    const int wide = (n + 31) & ~31;
+    if (2 * wide <= THREADS && n > 0) {
+        const int shares = THREADS / wide, share = (int)threadIdx.x / wide, i = (int)threadIdx.x % wide;
+        const unsigned long long key = i < n ? sh.key[i] : 0ull;
+        if (share < shares && i < n) atomicAdd(&sh.rank[i], above(key, pairs * share / shares, pairs * (share + 1) / shares));
+        __syncthreads();
+        if (share == 0 && i < n && sh.rank[i] < n_best) put(sh.rank[i], key);
+    } else {
+        for (int i = threadIdx.x; i < n; i += THREADS) {
+            const unsigned long long key = sh.key[i];
+            const int rank = above(key, 0, pairs);
+            if (rank < n_best) put(rank, key);
+        }
     }
     for (int i = n + (int)threadIdx.x; i < n_best; i += THREADS) put(i, 0ull);
 }
@@ -485,20 +586,24 @@ struct RowResult {  // what is written once a row's sums are known
 };
 __device__ __forceinline__ RowResult row_result(const Sums& total) { return RowResult{total.reference, log2f(total.sum), total.sum == 0.f}; }
 
-template <class T>
-__device__ __forceinline__ void write_row(const Scores& s, const Out& out, size_t r, const Row<T>& row, const Sums& total, const RowResult& res) {
-    const float entropy = res.empty ? 0.f : (res.log_total - total.weighted / total.sum) * kLn2;
-    const int t = s.target ? s.target[r] : -1;
-    float log_prob = 0.f, counted = 0.f;
-    if (t >= 0 && t < s.cols) {
-        const float x = row.at(t);
-        log_prob = x == -INFINITY ? -INFINITY : fmaf(x - total.reference, s.scale, -res.log_total * kLn2);
-        counted = x == -INFINITY ? 0.f : 1.f;
+struct Target {
+    bool asked;
+    float x;  // -inf: not live
+    __device__ __forceinline__ Target() : asked(false), x(-INFINITY) {}
+    template <class T>
+    __device__ __forceinline__ Target(const Scores& s, size_t r, const Row<T>& row) {
+        const int t = s.target ? s.target[r] : -1;
+        asked = t >= 0 && t < s.cols;
+        x = asked ? row.at(t) : -INFINITY;
     }
-    out.log_prob[r] = log_prob;
+};
+__device__ __forceinline__ void write_row(const Scores& s, const Out& out, size_t r, const Target& target, const Sums& total, const RowResult& res) {
+    const float entropy = res.empty ? 0.f : (res.log_total - total.weighted / total.sum) * kLn2;
+    const bool none = target.x == -INFINITY;
+    out.log_prob[r] = !target.asked ? 0.f : none ? -INFINITY : fmaf(target.x - total.reference, s.scale, -res.log_total * kLn2);
     out.entropy[r] = entropy;
     out.log_sum[r] = res.empty ? -INFINITY : fmaf(total.reference, s.scale, res.log_total * kLn2);
-    out.row_state[r] = make_float4(res.empty ? 0.f : total.reference, res.empty ? 0.f : res.log_total, entropy, counted);
+    out.row_state[r] = make_float4(res.empty ? 0.f : total.reference, res.empty ? 0.f : res.log_total, entropy, none ? 0.f : 1.f);
 }
 __device__ __forceinline__ void write_best(const Scores& s, const Out& out, size_t r, const RowResult& res, int rank, unsigned long long key) {
     const size_t at = r * (size_t)out.n_best + rank;
@@ -520,12 +625,12 @@ struct Parts {
 // are raised to kLow first, so that -inf makes no NaN of e d; where the largest score is no further than 2^64 above kLow that
 // would count them, and add_exactly does the part again.
 template <int THREADS, class T>
-__device__ __forceinline__ Sums add_part(const Row<T>& row, int v0, int v1, float s2, bool keep_groups, float* group_max, float& largest) {
+__device__ __forceinline__ Sums add_part(const Row<T>& row, int v0, int v1, float s2, float* groups, float& largest) {
     using W = Words<T>;
     float reference = W::kLow, r2 = 0.f;  // until a score is above kLow nothing counts
     float sum[2] = {}, weighted[2] = {};
-    int group = threadIdx.x;
-    for (int base = v0 + (int)threadIdx.x; base < v1; base += THREADS * kGroup, group += THREADS) {
+    int at = threadIdx.x & 31;
+    for (int base = v0 + (int)threadIdx.x; base < v1; base += THREADS * kGroup, at += 32) {
         Vector raw[kGroup];
         row.template load_group<THREADS>(base, v1, raw);
         uint32_t top = W::kNone;
@@ -535,7 +640,7 @@ __device__ __forceinline__ Sums add_part(const Row<T>& row, int v0, int v1, floa
             for (int i = 0; i < 4; ++i) top = W::larger(top, raw[u].w[i]);
         const float above = W::largest(top);
         largest = fmaxf(largest, above);
-        if (keep_groups) group_max[group] = above;
+        if (groups) groups[at] = above;
         if (above > reference) {
             reference = above;
             const float to = above * s2, d = fminf(fmaxf(r2 - to, kFarBelow), 0.f), c = ex2(d);
@@ -575,63 +680,34 @@ __device__ __noinline__ Sums add_exactly(const Row<T>& row, int v0, int v1, floa
 }
 
 template <class T, int THREADS>
-static __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_log_probs(Scores s, Out out, Parts parts) {
+static __global__ void __launch_bounds__(THREADS, THREADS == 128 ? 8 : 1024 / THREADS) k_log_probs(Scores s, Out out, Parts parts) {
     using W = Words<T>;
-    constexpr int V = Row<T>::V;
     __shared__ Shared<THREADS> sh;
     grid_dependency_sync();
     const uint32_t r = blockIdx.x / (uint32_t)parts.count, part = blockIdx.x % (uint32_t)parts.count;
     const Row<T> row(s, r);
     const int k = out.n_best;
     const int v0 = min(row.n_vectors, (int)part * parts.vectors), v1 = min(row.n_vectors, v0 + parts.vectors);
+    const bool writes = threadIdx.x == THREADS - 32;  // not in the warp that looks for the threshold
+    const Target target = writes && parts.count == 1 ? Target(s, r, row) : Target();
     float largest = -INFINITY;
     // a scale so large that kLow has no finite exponent is taken the long way
     const bool usual = fabsf(W::kLow * s.s2) < 1e37f;
-    Sums total = join_block<THREADS>(add_part<THREADS, T>(row, v0, v1, s.s2, k > 0, sh.group_max, largest), s.s2, sh);
+    Sums total = join_block<THREADS>(add_part<THREADS, T>(row, v0, v1, s.s2, k > 0 ? sh.groups[threadIdx.x / 32] : nullptr, largest), s.s2, sh);
     if (!usual || !((total.reference - W::kLow) * s.s2 > 64.f) || total.reference >= 1e37f / s.s2) {
         __syncthreads();
         total = join_block<THREADS>(add_exactly<THREADS, T>(row, v0, v1, s.s2), s.s2, sh);
     }
     const RowResult res = row_result(total);
-    if (threadIdx.x == 0) {
-        if (parts.count == 1) write_row(s, out, r, row, total, res);
+    if (writes) {
+        if (parts.count == 1) write_row(s, out, r, target, total, res);
         else parts.sums[blockIdx.x] = make_float4(total.reference, total.sum, total.weighted, 0.f);
     }
     if (k == 0) return;
     const uint32_t threshold = first_threshold<THREADS>(order_key(largest), k, sh);
-    // the groups that reach it, of these the vectors, of these the columns: each time a list that the block shares out anew
-    int group = threadIdx.x;
-    for (int base = v0 + (int)threadIdx.x; base < v1; base += THREADS * kGroup, group += THREADS)
-        if (order_key(sh.group_max[group]) >= threshold) {
-            const int at = atomicAdd(&sh.hits, 1);
-            if (at < kCandidates) sh.hit[at] = base;
-        }
+    collect<THREADS, T>(row, v0, v1, threshold, sh);
     __syncthreads();
-    const int hits = sh.hits;
-    if (hits <= kCandidates) {
-        int* const reached = reinterpret_cast<int*>(sh.group_max);
-        constexpr int kMost = kGroup * (kCandidates < THREADS * kGroupsPerThread<THREADS> ? kCandidates : THREADS * kGroupsPerThread<THREADS>);
-        static_assert(sizeof(sh.group_max) >= sizeof(int) * kMost, "a list of vectors takes the groups' place");
-        for (int i = threadIdx.x; i < hits * kGroup; i += THREADS) {
-            const int v = sh.hit[i / kGroup] + i % kGroup * THREADS;
-            if (v >= v1) continue;
-            const Vector raw = row.load(v);
-            const float top = W::largest(W::larger(W::larger(raw.w[0], raw.w[1]), W::larger(raw.w[2], raw.w[3])));
-            if (order_key(top) >= threshold) reached[atomicAdd(&sh.vectors, 1)] = v;
-        }
-        __syncthreads();
-        const int columns = sh.vectors * V;
-        for (int i = threadIdx.x; i < columns; i += THREADS) {
-            const int c = row.first_column(reached[i / V]) + i % V;
-            const uint32_t key = c >= 0 ? order_key(row.at(c)) : 0u;
-            if (key >= threshold) {
-                const int at = atomicAdd(&sh.count, 1);
-                if (at < kCandidates) sh.key[at] = candidate(key, c);
-            }
-        }
-        __syncthreads();
-    }
-    if (hits > kCandidates || sh.count > kCandidates) select_exactly<THREADS, T>(row, v0, v1, k, sh);
+    if (sh.overflow || sh.count > kCandidates) select_exactly<THREADS, T>(row, v0, v1, k, sh);
     else thin_candidates<THREADS>(k, sh);
     if (parts.count == 1) {
         rank_candidates<THREADS>(k, sh, [&](int rank, unsigned long long key) { write_best(s, out, r, res, rank, key); });
@@ -642,40 +718,53 @@ static __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_log_probs(Sc
 }
 
 // One block a row: the parts' sums joined in order, and the best of their lists.
-constexpr int kJoinThreads = 256;
-template <class T>
-static __global__ void __launch_bounds__(kJoinThreads) k_join_parts(Scores s, Out out, Parts parts) {
-    __shared__ Shared<kJoinThreads> sh;
+template <class T, int THREADS>
+static __global__ void __launch_bounds__(THREADS) k_join_parts(Scores s, Out out, Parts parts) {
+    __shared__ Shared<THREADS> sh;
     grid_dependency_sync();
     const size_t r = blockIdx.x;
     const Row<T> row(s, r);
+    const bool writes = threadIdx.x == THREADS - 32;
+    const Target target = writes ? Target(s, r, row) : Target();
     Sums sums = none_yet();
-    for (int i = threadIdx.x; i < parts.count; i += kJoinThreads) {
+    for (int i = threadIdx.x; i < parts.count; i += THREADS) {
         const float4 p = parts.sums[r * parts.count + i];
         sums.join(Sums{p.x, p.y, p.z}, s.s2);
     }
-    const Sums total = join_block<kJoinThreads>(sums, s.s2, sh);
+    const Sums total = join_block<THREADS>(sums, s.s2, sh);
     const RowResult res = row_result(total);
-    if (threadIdx.x == 0) write_row(s, out, r, row, total, res);
+    if (writes) write_row(s, out, r, target, total, res);
     const int k = out.n_best;
     if (k == 0) return;
     const unsigned long long* const keys = parts.keys + r * (size_t)parts.count * k;
     const int n = parts.count * k;
     // The lists are in order: `reach` parts whose `depth`-th best reaches a threshold have k keys that do.  The depth is such that
-    // half of the parts are asked for, and a warp follows a list as far as it reaches.
+    // half of the parts are asked for; neighbouring parts go to different warps, which first_threshold takes as they come.
     const int depth = min(k, max(1, (2 * k + parts.count - 1) / parts.count)), reach = (k + depth - 1) / depth;
     uint32_t largest = 0;
-    for (int i = threadIdx.x; i < parts.count; i += kJoinThreads) largest = max(largest, (uint32_t)(keys[(size_t)i * k + depth - 1] >> 32));
-    const uint32_t threshold = first_threshold<kJoinThreads>(largest, reach, sh);
-    for (int i = threadIdx.x / 32; i < parts.count; i += kJoinThreads / 32)
-        for (int j = threadIdx.x & 31; j < k; j += 32) {
-            const unsigned long long key = keys[(size_t)i * k + j];
-            if ((uint32_t)(key >> 32) < threshold) break;
-            const int at = atomicAdd(&sh.count, 1);
-            if (at < kCandidates) sh.key[at] = key;
+    constexpr int kJoinWarps = THREADS / 32;
+    for (int i = (threadIdx.x & 31) * kJoinWarps + threadIdx.x / 32; i < parts.count; i += THREADS)
+        largest = max(largest, (uint32_t)(keys[(size_t)i * k + depth - 1] >> 32));
+    const uint32_t threshold = first_threshold<THREADS>(largest, reach, sh);
+    for (int i = threadIdx.x / 32; i < parts.count; i += kJoinWarps) {
+        unsigned long long key[kMaxBest / 32];
+        int length = 0;
+#pragma unroll
+        for (int j = 0; j < kMaxBest / 32; ++j) {
+            const int at = 32 * j + ((int)threadIdx.x & 31);
+            key[j] = at < k ? keys[(size_t)i * k + at] : 0ull;
         }
+#pragma unroll
+        for (int j = 0; j < kMaxBest / 32; ++j) length += __popc(__ballot_sync(~0u, (uint32_t)(key[j] >> 32) >= threshold));
+        const int room = reserve(sh, length);  // the list is in order: those that reach it come first
+#pragma unroll
+        for (int j = 0; j < kMaxBest / 32; ++j) {
+            const int at = 32 * j + ((int)threadIdx.x & 31);
+            if (at < length && room + at < kCandidates) sh.key[room + at] = key[j];
+        }
+    }
     __syncthreads();
-    thin_candidates<kJoinThreads>(k, sh);
+    thin_candidates<THREADS>(k, sh);
     if (sh.count > kCandidates) {
         // Equal scores in every part: the lists are in order, so a binary search over key and column finds how far each counts.
         unsigned long long low = (unsigned long long)threshold << 32, high = ~0ull;  // at least k keys are >= low
@@ -685,7 +774,7 @@ static __global__ void __launch_bounds__(kJoinThreads) k_join_parts(Scores s, Ou
             if (threadIdx.x == 0) sh.count = 0;
             __syncthreads();
             int mine = 0;
-            for (int i = threadIdx.x; i < n; i += kJoinThreads) mine += keys[i] >= mid;
+            for (int i = threadIdx.x; i < n; i += THREADS) mine += keys[i] >= mid;
             if (mine) atomicAdd(&sh.count, mine);
             __syncthreads();
             if (sh.count >= k) low = mid;
@@ -694,11 +783,11 @@ static __global__ void __launch_bounds__(kJoinThreads) k_join_parts(Scores s, Ou
         __syncthreads();
         if (threadIdx.x == 0) sh.count = 0;
         __syncthreads();
-        for (int i = threadIdx.x; i < n; i += kJoinThreads)
+        for (int i = threadIdx.x; i < n; i += THREADS)
             if (keys[i] >= low) sh.key[atomicAdd(&sh.count, 1)] = keys[i];  // keys differ: k of them
         __syncthreads();
     }
-    rank_candidates<kJoinThreads>(k, sh, [&](int rank, unsigned long long key) { write_best(s, out, r, res, rank, key); });
+    rank_candidates<THREADS>(k, sh, [&](int rank, unsigned long long key) { write_best(s, out, r, res, rank, key); });
 }
 
 // The gradient: every score is read once and every gradient written once.
