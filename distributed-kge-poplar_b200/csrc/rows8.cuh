@@ -43,104 +43,252 @@ __device__ __forceinline__ uint32_t finite_magnitude(float x) {
     const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
     return b < 0x7f800000u ? b : 0u;
 }
-// Four values as e4m3, NaN for what is not finite (the conversion would saturate an infinity).
-__device__ __forceinline__ uint32_t to_e4m3x4(const float (&x)[4], float inverse) {
-    uint16_t lo, hi;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(x[1] * inverse), "f"(x[0] * inverse));
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(x[3] * inverse), "f"(x[2] * inverse));
-    uint32_t w = (uint32_t)lo | (uint32_t)hi << 16;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if ((__float_as_uint(x[i]) & 0x7f800000u) == 0x7f800000u) w = (w & ~(0xffu << (8 * i))) | (uint32_t)kNan << (8 * i);
+__device__ __forceinline__ uint32_t to_e4m3x2(float lo, float hi) {
+    uint16_t w;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(w) : "f"(hi), "f"(lo));
     return w;
 }
+// Sixteen values times `inverse` as e4m3.  The conversion saturates an infinity, so where some value is not finite (`special`) those
+// become NaN one by one.
+__device__ __forceinline__ uint4 to_e4m3x16(const float (&v)[16], float inverse, bool special) {
+    uint32_t w[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+        w[q] = to_e4m3x2(v[4 * q] * inverse, v[4 * q + 1] * inverse) | to_e4m3x2(v[4 * q + 2] * inverse, v[4 * q + 3] * inverse) << 16;
+    if (special) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if ((__float_as_uint(v[i]) & 0x7f800000u) == 0x7f800000u) w[i / 4] = (w[i / 4] & ~(0xffu << (8 * (i % 4)))) | (uint32_t)kNan << (8 * (i % 4));
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
 
-// A thread takes 16 consecutive values: 8 lanes a block, a warp the 4 blocks whose bytes lie side by side.
+// Sixteen values as they lie in memory: 8 words of two or 16 of one.
 template <class T>
-static __global__ void __launch_bounds__(256) k_quantise_rows(const T* __restrict__ x, size_t rows, size_t cols, long long stride, size_t groups,
-                                                              uint8_t* __restrict__ values, uint8_t* __restrict__ exponents) {
-    const size_t unit = (size_t)blockIdx.x * 8 + threadIdx.x / 32;  // (row, group), rows rounded up to 128
-    const size_t r = unit / groups, group = unit % groups;
-    const int lane = threadIdx.x & 31;
-    const size_t row_tiles = (rows + 127) / 128;
-    if (r >= row_tiles * 128) return;
-    uint32_t* const bytes = reinterpret_cast<uint32_t*>(exponents + ((r / 128) * groups + group) * kGroupBytes + (r % 32) * 16 + (r % 128) / 32 * 4);
-    if (r >= rows) {
-        if (lane == 0) *bytes = 0x01010101u * kOne;
-        return;
+struct Sixteen {
+    static constexpr int kPer = lp::Words<T>::kPer, kWords = 16 / kPer;
+    uint32_t w[kWords];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) w[i] = 0;
     }
-    const size_t c0 = group * (4 * kBlock) + lane * 16, ld = (cols + 15) / 16 * 16;
-    const T* const src = x + (long long)r * stride + c0;
-    float v[16];
-    if (c0 + 16 <= cols && (reinterpret_cast<uintptr_t>(src) & 15u) == 0) {
-        constexpr int V = 16 / (int)sizeof(T);
+    // The values from p on, `live` of them and zeros after; `first` and `end` are where the whole matrix lies.  Off a 16-byte boundary the
+    // vectors around the values are read and shifted into place (512 x 100 001 bf16 values: 61 us read value by value).
+    __device__ __forceinline__ void load(const T* p, int live, const T* first, const T* end) {
+        const uint32_t off = (uint32_t)(reinterpret_cast<uintptr_t>(p) & 15u);
+        const uint4* const q = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(p) - off);
+        if (live >= 16 && off == 0) {
 #pragma unroll
-        for (int q = 0; q < 16 / V; ++q) {
-            float part[V];
-            const uint4 t = reinterpret_cast<const uint4*>(src)[q];
-            lp::unpack<T>(lp::Vector{{t.x, t.y, t.z, t.w}}, part);
+            for (int i = 0; i < kWords / 4; ++i) {
+                const uint4 t = q[i];
+                w[4 * i] = t.x, w[4 * i + 1] = t.y, w[4 * i + 2] = t.z, w[4 * i + 3] = t.w;
+            }
+        } else if (live >= 16 && reinterpret_cast<const T*>(q) >= first && reinterpret_cast<const T*>(q + kWords / 4 + 1) <= end) {
+            uint32_t a[kWords + 4];
 #pragma unroll
-            for (int j = 0; j < V; ++j) v[q * V + j] = part[j];
+            for (int i = 0; i <= kWords / 4; ++i) {
+                const uint4 t = q[i];
+                a[4 * i] = t.x, a[4 * i + 1] = t.y, a[4 * i + 2] = t.z, a[4 * i + 3] = t.w;
+            }
+            if (off & 8u) {
+#pragma unroll
+                for (int i = 0; i < kWords + 2; ++i) a[i] = a[i + 2];
+            }
+            if (off & 4u) {
+#pragma unroll
+                for (int i = 0; i < kWords + 1; ++i) a[i] = a[i + 1];
+            }
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) w[i] = __funnelshift_r(a[i], a[i + 1], (off & 3u) * 8u);
+        } else {
+            clear();
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+                if (j < live) w[j / kPer] |= lp::Row<T>::bits(p + j) << (kPer == 2 ? 16 * (j & 1) : 0);
         }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] = c0 + j < cols ? lp::as_float(src[j]) : 0.f;
     }
-    uint32_t largest = 0;
+    // The largest magnitude, as the bits of an fp32; infinities and NaN are above all others.
+    __device__ __forceinline__ uint32_t largest() const {
+        if constexpr (kPer == 1) {
+            uint32_t m = 0;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) largest = max(largest, finite_magnitude(v[j]));
+            for (int i = 0; i < kWords; ++i) m = max(m, w[i] & 0x7fffffffu);
+            return m;
+        } else {
+            uint32_t m = 0;
 #pragma unroll
-    for (int o = 4; o > 0; o >>= 1) largest = max(largest, __shfl_xor_sync(~0u, largest, o));
-    const int byte = exponent_byte(largest);
-    const float inverse = inverse_scale(byte);
-    uint32_t four = (uint32_t)byte << (8 * (lane / 8));
-    four |= __shfl_xor_sync(~0u, four, 8);
-    four |= __shfl_xor_sync(~0u, four, 16);
-    if (lane == 0) *bytes = four;
-    if (c0 < ld) {
-        uint4 q;
-        q.x = to_e4m3x4({v[0], v[1], v[2], v[3]}, inverse);
-        q.y = to_e4m3x4({v[4], v[5], v[6], v[7]}, inverse);
-        q.z = to_e4m3x4({v[8], v[9], v[10], v[11]}, inverse);
-        q.w = to_e4m3x4({v[12], v[13], v[14], v[15]}, inverse);
-        *reinterpret_cast<uint4*>(values + r * ld + c0) = q;
+            for (int i = 0; i < kWords; ++i) m = larger_halves(m, w[i] & 0x7fff7fffu);
+            return magnitude(max(m & 0xffffu, m >> 16));
+        }
+    }
+    static __device__ __forceinline__ uint32_t larger_halves(uint32_t a, uint32_t b) {
+        uint32_t r;
+        asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
+    }
+    static __device__ __forceinline__ uint32_t magnitude(uint32_t half) { return __float_as_uint(lp::Words<T>::floats(half).x); }
+    __device__ __forceinline__ void floats(float (&v)[16]) const {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+            const float2 t = lp::Words<T>::floats(w[i]);
+            v[kPer * i] = t.x;
+            if (kPer == 2) v[kPer * i + 1] = t.y;
+        }
+    }
+};
+
+// A thread takes 16 consecutive values: 8 lanes a block, a warp the 4 blocks whose bytes lie side by side.  A warp does kUnits such
+// units, all fetched before the first is worked on: bound by memory, it needs that much in flight.
+constexpr int kUnits = 4;
+template <class T>
+static __global__ void __launch_bounds__(256) k_quantise_rows(const T* __restrict__ x, uint32_t rows, size_t cols, long long stride, uint32_t groups, uint32_t units,
+                                                              uint8_t* __restrict__ values, uint8_t* __restrict__ exponents) {
+    grid_dependency_sync();
+    const int lane = threadIdx.x & 31;
+    const size_t ld = (cols + 15) / 16 * 16;
+    const uint32_t unit0 = (blockIdx.x * 8 + threadIdx.x / 32) * kUnits;  // (row, group), rows rounded up to 128
+    const T* const end = x + (long long)(rows - 1) * stride + (long long)cols;
+    Sixteen<T> raw[kUnits];
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+        const uint32_t r = (unit0 + u) / groups, group = (unit0 + u) % groups;
+        const size_t c0 = (size_t)group * (4 * kBlock) + lane * 16;
+        if (unit0 + u < units && r < rows && c0 < cols) raw[u].load(x + (long long)r * stride + c0, (int)min((size_t)16, cols - c0), x, end);
+        else raw[u].clear();
+    }
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+        if (unit0 + u >= units) return;
+        const uint32_t r = (unit0 + u) / groups, group = (unit0 + u) % groups;
+        float v[16];
+        raw[u].floats(v);
+        uint32_t largest = raw[u].largest();
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) largest = max(largest, __shfl_xor_sync(~0u, largest, o));
+        const bool special = largest >= 0x7f800000u;
+        if (__any_sync(~0u, special)) {
+            uint32_t finite = 0;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) finite = max(finite, finite_magnitude(v[j]));
+#pragma unroll
+            for (int o = 4; o > 0; o >>= 1) finite = max(finite, __shfl_xor_sync(~0u, finite, o));
+            largest = finite;
+        }
+        const int byte = exponent_byte(largest);
+        uint32_t four = (uint32_t)byte << (8 * (lane / 8));
+        four |= __shfl_xor_sync(~0u, four, 8);
+        four |= __shfl_xor_sync(~0u, four, 16);
+        if (lane == 0) *reinterpret_cast<uint32_t*>(exponents + ((size_t)(r / 128) * groups + group) * kGroupBytes + (r % 32) * 16 + (r % 128) / 32 * 4) = four;
+        const size_t c0 = (size_t)group * (4 * kBlock) + lane * 16;
+        if (r < rows && c0 < ld) *reinterpret_cast<uint4*>(values + (size_t)r * ld + c0) = to_e4m3x16(v, inverse_scale(byte), special);
     }
 }
 
-// The columns of x as rows: a block is 128 rows of x in one column.  64 columns and 128 rows to a thread block; a thread keeps 32
-// rows of its column, so x is read along its rows and each thread writes 32 bytes side by side.
+// The columns of x as rows: a block is 128 rows of x in one column.  64 columns and 128 rows to a thread block; a warp takes 16 rows,
+// a thread two columns of them (neighbours where two fit a word), so that x is read along its rows, 128 bytes a warp; the bytes
+// are turned in shared memory and written 128 side by side.
 constexpr int kTurnCols = 64;
 template <class T>
 static __global__ void __launch_bounds__(256) k_quantise_columns(const T* __restrict__ x, size_t rows, size_t cols, long long stride, size_t groups,
                                                                  uint8_t* __restrict__ values, uint8_t* __restrict__ exponents) {
-    __shared__ uint32_t s_largest[4][kTurnCols];
+    constexpr int kPer = lp::Words<T>::kPer;
+    constexpr int kPitch = kBlock + 16;
+    __shared__ uint32_t s_largest[8][kTurnCols];
+    __shared__ alignas(16) uint8_t s_out[kTurnCols * kPitch];
+    grid_dependency_sync();
     const size_t blocks = (rows + kBlock - 1) / kBlock, all_blocks = groups * 4;
     const size_t tile = blockIdx.x / all_blocks, block = blockIdx.x % all_blocks;  // columns are rounded up to 128
-    const int tc = threadIdx.x % kTurnCols, quarter = threadIdx.x / kTurnCols;
-    const size_t c = tile * kTurnCols + tc, r0 = block * kBlock + (size_t)quarter * 32, ld = (rows + 15) / 16 * 16;
-    float v[32];
-    uint32_t largest = 0;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+    const size_t c0 = tile * kTurnCols, r0 = block * kBlock + (size_t)warp * 16, ld = (rows + 15) / 16 * 16;
+    const int own[2] = {kPer == 2 ? 2 * lane : lane, kPer == 2 ? 2 * lane + 1 : lane + 32};  // this thread's columns of the tile
+    float v[2][16];
+    const bool inside = c0 >= 1 && c0 + kTurnCols + 1 <= cols;  // a word to either side is the row's too
+    if (kPer == 2 && (inside || c0 + kTurnCols <= cols)) {
+        uint32_t word[16], next[16];
+        bool off[16];
 #pragma unroll
-    for (int j = 0; j < 32; ++j) {
-        v[j] = c < cols && r0 + j < rows ? lp::as_float(x[(long long)(r0 + j) * stride + (long long)c]) : 0.f;
-        largest = max(largest, finite_magnitude(v[j]));
+        for (int j = 0; j < 16; ++j) {
+            const T* const p = x + (long long)(r0 + j) * stride + (long long)c0 + own[0];
+            off[j] = (reinterpret_cast<uintptr_t>(p) & 2u) != 0;
+            word[j] = next[j] = 0;
+            if (r0 + j < rows) {
+                if (!off[j]) {
+                    word[j] = *reinterpret_cast<const uint32_t*>(p);
+                } else if (inside) {  // the upper half of this word and the lower one of the next lane's
+                    word[j] = *reinterpret_cast<const uint32_t*>(p - 1);
+                    if (lane == 31) next[j] = *reinterpret_cast<const uint32_t*>(p + 1);
+                } else {
+                    word[j] = lp::Row<T>::bits(p) | lp::Row<T>::bits(p + 1) << 16;
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            uint32_t w = word[j];
+            if (inside) {
+                const uint32_t after = __shfl_down_sync(~0u, w, 1);
+                if (off[j]) w = __funnelshift_r(w, lane == 31 ? next[j] : after, 16);
+            }
+            const float2 t = lp::Words<T>::floats(w);
+            v[0][j] = t.x, v[1][j] = t.y;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const size_t c = c0 + own[h];
+                v[h][j] = c < cols && r0 + j < rows ? lp::as_float(x[(long long)(r0 + j) * stride + (long long)c]) : 0.f;
+            }
     }
-    s_largest[quarter][tc] = largest;
-    __syncthreads();
-    largest = max(max(s_largest[0][tc], s_largest[1][tc]), max(s_largest[2][tc], s_largest[3][tc]));
-    const int byte = block < blocks ? exponent_byte(largest) : kOne;
-    if (quarter == 0) exponents[((c / 128) * groups + block / 4) * kGroupBytes + (c % 32) * 16 + (c % 128) / 32 * 4 + block % 4] = (uint8_t)byte;
-    if (c >= cols) return;
-    const float inverse = inverse_scale(byte);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        if (r0 + 16 * h >= ld) continue;
-        uint4 q;
-        q.x = to_e4m3x4({v[16 * h], v[16 * h + 1], v[16 * h + 2], v[16 * h + 3]}, inverse);
-        q.y = to_e4m3x4({v[16 * h + 4], v[16 * h + 5], v[16 * h + 6], v[16 * h + 7]}, inverse);
-        q.z = to_e4m3x4({v[16 * h + 8], v[16 * h + 9], v[16 * h + 10], v[16 * h + 11]}, inverse);
-        q.w = to_e4m3x4({v[16 * h + 12], v[16 * h + 13], v[16 * h + 14], v[16 * h + 15]}, inverse);
-        *reinterpret_cast<uint4*>(values + c * ld + r0 + 16 * h) = q;
+        uint32_t largest = 0;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) largest = max(largest, __float_as_uint(v[h][j]) & 0x7fffffffu);
+        s_largest[warp][own[h]] = largest;
+    }
+    __syncthreads();
+    int byte[2];
+    bool special[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        uint32_t largest = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) largest = max(largest, s_largest[i][own[h]]);
+        special[h] = largest >= 0x7f800000u;
+        byte[h] = (int)largest;
+    }
+    if (__syncthreads_or(special[0] || special[1])) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            uint32_t finite = 0;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) finite = max(finite, finite_magnitude(v[h][j]));
+            s_largest[warp][own[h]] = finite;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            uint32_t finite = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) finite = max(finite, s_largest[i][own[h]]);
+            byte[h] = (int)finite;
+        }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        byte[h] = block < blocks ? exponent_byte((uint32_t)byte[h]) : kOne;
+        const size_t c = c0 + own[h];
+        if (warp == 0) exponents[((c / 128) * groups + block / 4) * kGroupBytes + (c % 32) * 16 + (c % 128) / 32 * 4 + block % 4] = (uint8_t)byte[h];
+        *reinterpret_cast<uint4*>(s_out + own[h] * kPitch + warp * 16) = to_e4m3x16(v[h], inverse_scale(byte[h]), special[h]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int column = (int)threadIdx.x / 8 + 32 * h, piece = (int)threadIdx.x % 8;
+        const size_t c = c0 + column, r = block * kBlock + (size_t)piece * 16;
+        if (c < cols && r < ld) *reinterpret_cast<uint4*>(values + c * ld + r) = *reinterpret_cast<const uint4*>(s_out + column * kPitch + piece * 16);
     }
 }
 
