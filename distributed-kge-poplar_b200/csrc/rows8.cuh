@@ -137,29 +137,28 @@ struct Sixteen {
     }
 };
 
-// A thread takes 16 consecutive values: 8 lanes a block, a warp the 4 blocks whose bytes lie side by side.  A warp does kUnits such
-// units, all fetched before the first is worked on: bound by memory, it needs that much in flight.
+// Eight lanes take a block, 16 consecutive values each, and a warp kUnits times four blocks, all fetched before the first is worked
+// on: bound by memory, it needs that much in flight.
 constexpr int kUnits = 4;
 template <class T>
-static __global__ void __launch_bounds__(256) k_quantise_rows(const T* __restrict__ x, uint32_t rows, size_t cols, long long stride, uint32_t groups, uint32_t units,
-                                                              uint8_t* __restrict__ values, uint8_t* __restrict__ exponents) {
+static __global__ void __launch_bounds__(256) k_quantise_rows(const T* __restrict__ x, uint32_t rows, size_t cols, long long stride, uint32_t blocks, uint32_t groups,
+                                                              uint32_t units, uint8_t* __restrict__ values, uint8_t* __restrict__ exponents) {
     grid_dependency_sync();
     const int lane = threadIdx.x & 31;
     const size_t ld = (cols + 15) / 16 * 16;
-    const uint32_t unit0 = (blockIdx.x * 8 + threadIdx.x / 32) * kUnits;  // (row, group), rows rounded up to 128
+    const uint32_t unit0 = (blockIdx.x * 8 + threadIdx.x / 32) * (4 * kUnits) + lane / 8;  // (row, block), rows rounded up to 128
     const T* const end = x + (long long)(rows - 1) * stride + (long long)cols;
     Sixteen<T> raw[kUnits];
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) {
-        const uint32_t r = (unit0 + u) / groups, group = (unit0 + u) % groups;
-        const size_t c0 = (size_t)group * (4 * kBlock) + lane * 16;
-        if (unit0 + u < units && r < rows && c0 < cols) raw[u].load(x + (long long)r * stride + c0, (int)min((size_t)16, cols - c0), x, end);
+        const uint32_t unit = unit0 + 4 * u, r = unit / blocks, block = unit - r * blocks;
+        const size_t c0 = (size_t)block * kBlock + (lane & 7) * 16;
+        if (unit < units && r < rows && c0 < cols) raw[u].load(x + (long long)r * stride + c0, (int)min((size_t)16, cols - c0), x, end);
         else raw[u].clear();
     }
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) {
-        if (unit0 + u >= units) return;
-        const uint32_t r = (unit0 + u) / groups, group = (unit0 + u) % groups;
+        const uint32_t unit = unit0 + 4 * u, r = unit / blocks, block = unit - r * blocks;
         float v[16];
         raw[u].floats(v);
         uint32_t largest = raw[u].largest();
@@ -174,25 +173,28 @@ static __global__ void __launch_bounds__(256) k_quantise_rows(const T* __restric
             for (int o = 4; o > 0; o >>= 1) finite = max(finite, __shfl_xor_sync(~0u, finite, o));
             largest = finite;
         }
+        if (unit >= units) continue;
         const int byte = exponent_byte(largest);
-        uint32_t four = (uint32_t)byte << (8 * (lane / 8));
-        four |= __shfl_xor_sync(~0u, four, 8);
-        four |= __shfl_xor_sync(~0u, four, 16);
-        if (lane == 0) *reinterpret_cast<uint32_t*>(exponents + ((size_t)(r / 128) * groups + group) * kGroupBytes + (r % 32) * 16 + (r % 128) / 32 * 4) = four;
-        const size_t c0 = (size_t)group * (4 * kBlock) + lane * 16;
+        if ((lane & 7) == 0) {
+            uint8_t* const bytes = exponents + (size_t)(r / 128) * groups * kGroupBytes + (r % 32) * 16 + (r % 128) / 32 * 4;
+            bytes[block / 4 * kGroupBytes + block % 4] = (uint8_t)byte;
+            for (uint32_t none = block + 1; block + 1 == blocks && none % 4 != 0; ++none) bytes[none / 4 * kGroupBytes + none % 4] = kOne;
+        }
+        const size_t c0 = (size_t)block * kBlock + (lane & 7) * 16;
         if (r < rows && c0 < ld) *reinterpret_cast<uint4*>(values + (size_t)r * ld + c0) = to_e4m3x16(v, inverse_scale(byte), special);
     }
 }
 
 // The columns of x as rows: a block is 128 rows of x in one column.  64 columns and 128 rows to a thread block; a warp takes 16 rows,
-// a thread two columns of them (neighbours where two fit a word), so that x is read along its rows, 128 bytes a warp; the bytes
-// are turned in shared memory and written 128 side by side.
+// a thread two columns of them: neighbours where two fit a word, so that a warp reads 128 bytes of a row at once (value by value
+// 512 x 100 001 bf16 values took 96 us, this COLS1).  Rows that begin inside a word get their pairs from two lanes' words.  The
+// bytes are turned in shared memory and written 128 side by side.
 constexpr int kTurnCols = 64;
 template <class T>
 static __global__ void __launch_bounds__(256) k_quantise_columns(const T* __restrict__ x, size_t rows, size_t cols, long long stride, size_t groups,
                                                                  uint8_t* __restrict__ values, uint8_t* __restrict__ exponents) {
-    constexpr int kPer = lp::Words<T>::kPer;
-    constexpr int kPitch = kBlock + 16;
+    using S = Sixteen<T>;
+    constexpr int kPer = S::kPer, kPitch = kBlock + 16;
     __shared__ uint32_t s_largest[8][kTurnCols];
     __shared__ alignas(16) uint8_t s_out[kTurnCols * kPitch];
     grid_dependency_sync();
@@ -201,94 +203,96 @@ static __global__ void __launch_bounds__(256) k_quantise_columns(const T* __rest
     const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
     const size_t c0 = tile * kTurnCols, r0 = block * kBlock + (size_t)warp * 16, ld = (rows + 15) / 16 * 16;
     const int own[2] = {kPer == 2 ? 2 * lane : lane, kPer == 2 ? 2 * lane + 1 : lane + 32};  // this thread's columns of the tile
-    float v[2][16];
-    const bool inside = c0 >= 1 && c0 + kTurnCols + 1 <= cols;  // a word to either side is the row's too
-    if (kPer == 2 && (inside || c0 + kTurnCols <= cols)) {
-        uint32_t word[16], next[16];
-        bool off[16];
+    const int live = r0 < rows ? (int)min((size_t)16, rows - r0) : 0;
+    const T* const p = x + (long long)r0 * stride + (long long)c0 + own[0];
+    uint32_t w[kPer == 2 ? 16 : 32];  // two columns of 16 rows: side by side in a word, or one after the other
+    if (kPer == 2 && c0 >= 1 && c0 + kTurnCols + 1 <= cols) {  // a word to either side is the row's too
+        uint32_t next[16];
+        uint32_t off = 0;  // rows that begin inside a word
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-            const T* const p = x + (long long)(r0 + j) * stride + (long long)c0 + own[0];
-            off[j] = (reinterpret_cast<uintptr_t>(p) & 2u) != 0;
-            word[j] = next[j] = 0;
-            if (r0 + j < rows) {
-                if (!off[j]) {
-                    word[j] = *reinterpret_cast<const uint32_t*>(p);
-                } else if (inside) {  // the upper half of this word and the lower one of the next lane's
-                    word[j] = *reinterpret_cast<const uint32_t*>(p - 1);
-                    if (lane == 31) next[j] = *reinterpret_cast<const uint32_t*>(p + 1);
-                } else {
-                    word[j] = lp::Row<T>::bits(p) | lp::Row<T>::bits(p + 1) << 16;
-                }
-            }
+            const uintptr_t at = reinterpret_cast<uintptr_t>(p + (long long)j * stride);
+            const bool inside = (at & 2u) != 0;
+            off |= inside ? 1u << j : 0u;
+            const uint32_t* const word = reinterpret_cast<const uint32_t*>(at & ~(uintptr_t)3);
+            w[j] = j < live ? word[0] : 0u;
+            next[j] = inside && lane == 31 && j < live ? word[1] : 0u;
         }
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-            uint32_t w = word[j];
-            if (inside) {
-                const uint32_t after = __shfl_down_sync(~0u, w, 1);
-                if (off[j]) w = __funnelshift_r(w, lane == 31 ? next[j] : after, 16);
-            }
-            const float2 t = lp::Words<T>::floats(w);
-            v[0][j] = t.x, v[1][j] = t.y;
+            const uint32_t after = __shfl_down_sync(~0u, w[j], 1);
+            if (off >> j & 1u) w[j] = __funnelshift_r(w[j], lane == 31 ? next[j] : after, 16);
         }
     } else {
+        const bool here[2] = {c0 + own[0] < cols, c0 + own[1] < cols};
+        const int apart = own[1] - own[0];
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const size_t c = c0 + own[h];
-                v[h][j] = c < cols && r0 + j < rows ? lp::as_float(x[(long long)(r0 + j) * stride + (long long)c]) : 0.f;
-            }
+        for (int j = 0; j < 16; ++j) {
+            const uint32_t a = here[0] && j < live ? lp::Row<T>::bits(p + (long long)j * stride) : 0u;
+            const uint32_t b = here[1] && j < live ? lp::Row<T>::bits(p + (long long)j * stride + apart) : 0u;
+            if (kPer == 2) w[j] = a | b << 16;
+            else w[j] = a, w[(j + 16) % (kPer == 2 ? 16 : 32)] = b;
+        }
     }
+    if constexpr (kPer == 2) {
+        uint32_t m = 0;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        uint32_t largest = 0;
+        for (int j = 0; j < 16; ++j) m = S::larger_halves(m, w[j] & 0x7fff7fffu);
+        s_largest[warp][own[0]] = S::magnitude(m & 0xffffu);
+        s_largest[warp][own[1]] = S::magnitude(m >> 16);
+    } else {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) largest = max(largest, __float_as_uint(v[h][j]) & 0x7fffffffu);
-        s_largest[warp][own[h]] = largest;
+        for (int h = 0; h < 2; ++h) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) m = max(m, w[16 * h + j] & 0x7fffffffu);
+            s_largest[warp][own[h]] = m;
+        }
     }
+    const auto column = [&](int h, float (&v)[16]) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const float2 t = lp::Words<T>::floats(w[kPer == 2 ? j : 16 * h + j]);
+            v[j] = kPer == 2 && h ? t.y : t.x;
+        }
+    };
+    const auto block_largest = [&](int h) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = max(m, s_largest[i][own[h]]);
+        return m;
+    };
     __syncthreads();
-    int byte[2];
-    bool special[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        uint32_t largest = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) largest = max(largest, s_largest[i][own[h]]);
-        special[h] = largest >= 0x7f800000u;
-        byte[h] = (int)largest;
-    }
+    uint32_t largest[2] = {block_largest(0), block_largest(1)};
+    const bool special[2] = {largest[0] >= 0x7f800000u, largest[1] >= 0x7f800000u};
     if (__syncthreads_or(special[0] || special[1])) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            uint32_t finite = 0;
+            float v[16];
+            column(h, v);
+            uint32_t m = 0;
 #pragma unroll
-            for (int j = 0; j < 16; ++j) finite = max(finite, finite_magnitude(v[h][j]));
-            s_largest[warp][own[h]] = finite;
+            for (int j = 0; j < 16; ++j) m = max(m, finite_magnitude(v[j]));
+            s_largest[warp][own[h]] = m;
         }
         __syncthreads();
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            uint32_t finite = 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) finite = max(finite, s_largest[i][own[h]]);
-            byte[h] = (int)finite;
-        }
+        largest[0] = block_largest(0), largest[1] = block_largest(1);
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        byte[h] = block < blocks ? exponent_byte((uint32_t)byte[h]) : kOne;
+        const int byte = block < blocks ? exponent_byte(largest[h]) : kOne;
         const size_t c = c0 + own[h];
-        if (warp == 0) exponents[((c / 128) * groups + block / 4) * kGroupBytes + (c % 32) * 16 + (c % 128) / 32 * 4 + block % 4] = (uint8_t)byte[h];
-        *reinterpret_cast<uint4*>(s_out + own[h] * kPitch + warp * 16) = to_e4m3x16(v[h], inverse_scale(byte[h]), special[h]);
+        if (warp == 0) exponents[((c / 128) * groups + block / 4) * kGroupBytes + (c % 32) * 16 + (c % 128) / 32 * 4 + block % 4] = (uint8_t)byte;
+        float v[16];
+        column(h, v);
+        *reinterpret_cast<uint4*>(s_out + own[h] * kPitch + warp * 16) = to_e4m3x16(v, inverse_scale(byte), special[h]);
     }
     __syncthreads();
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        const int column = (int)threadIdx.x / 8 + 32 * h, piece = (int)threadIdx.x % 8;
-        const size_t c = c0 + column, r = block * kBlock + (size_t)piece * 16;
-        if (c < cols && r < ld) *reinterpret_cast<uint4*>(values + c * ld + r) = *reinterpret_cast<const uint4*>(s_out + column * kPitch + piece * 16);
+        const int row = (int)threadIdx.x / 8 + 32 * h, piece = (int)threadIdx.x % 8;
+        const size_t c = c0 + row, r = block * kBlock + (size_t)piece * 16;
+        if (c < cols && r < ld) *reinterpret_cast<uint4*>(values + c * ld + r) = *reinterpret_cast<const uint4*>(s_out + row * kPitch + piece * 16);
     }
 }
 
