@@ -198,8 +198,9 @@ static __global__ void __launch_bounds__(256) k_quantise_columns(const T* __rest
     __shared__ uint32_t s_largest[8][kTurnCols];
     __shared__ alignas(16) uint8_t s_out[kTurnCols * kPitch];
     grid_dependency_sync();
-    const size_t blocks = (rows + kBlock - 1) / kBlock, all_blocks = groups * 4;
-    const size_t tile = blockIdx.x / all_blocks, block = blockIdx.x % all_blocks;  // columns are rounded up to 128
+    const size_t blocks = (rows + kBlock - 1) / kBlock;
+    const size_t tiles = (cols + 127) / 128 * (128 / kTurnCols);  // columns are rounded up to 128
+    const size_t block = blockIdx.x / tiles, tile = blockIdx.x % tiles;  // neighbours read neighbouring parts of the same rows
     const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
     const size_t c0 = tile * kTurnCols, r0 = block * kBlock + (size_t)warp * 16, ld = (rows + 15) / 16 * 16;
     const int own[2] = {kPer == 2 ? 2 * lane : lane, kPer == 2 ? 2 * lane + 1 : lane + 32};  // this thread's columns of the tile
