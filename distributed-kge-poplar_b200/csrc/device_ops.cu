@@ -201,13 +201,16 @@ void quantise_rows(const void* x, int float_type, size_t rows, size_t cols, long
 namespace {
 
 struct ProductPlan {
-    int tile_m, m_tiles, n_tiles, blocks, splits;
+    int tile_m, m_tiles, n_tiles, blocks, splits, chunk;
 };
 ProductPlan product_plan(size_t m, size_t n, size_t k) {
     ProductPlan p;
-    p.tile_m = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128;
-    p.m_tiles = (int)((m + p.tile_m - 1) / p.tile_m);
     p.n_tiles = (int)((n + rows8::kTileN - 1) / rows8::kTileN);
+    p.tile_m = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : m <= 128 ? 128 : 256;
+    // where the sum has to be split, smaller tiles need half the parts and so half the partial sums
+    if (p.tile_m == 256 && (long long)((m + 255) / 256) * p.n_tiles < kSmCount / 2) p.tile_m = 128;
+    p.m_tiles = (int)((m + p.tile_m - 1) / p.tile_m);
+    p.chunk = (int)std::min<size_t>(p.n_tiles, std::max<size_t>(16, ((size_t)32 << 20) / (rows8::kTileN * rows8::value_stride(std::max<size_t>(k, 1)))));
     p.blocks = (int)rows8::blocks_of(k);
     const long long tiles = (long long)p.m_tiles * p.n_tiles;
     p.splits = (int)std::max<long long>(1, std::min<long long>(tiles ? kSmCount / tiles : 1, p.blocks / 4));
@@ -231,14 +234,16 @@ void launch_product(const CUtensorMap& a, const CUtensorMap& b, const rows8::Pro
     constexpr size_t smem = rows8::Tile<TM>::smem();
     allow_shared_memory<rows8::k_product8<TM, TOut>>(smem);
     const int work = g.n_tiles * g.m_tiles * g.splits;
-    rows8::k_product8<TM, TOut><<<std::min(work, kSmCount), rows8::Tile<TM>::kThreads, smem, stream>>>(a, b, g);
+    const cudaError_t err = launch_dependent(rows8::k_product8<TM, TOut>, dim3(std::min(work, kSmCount)), dim3(rows8::Tile<TM>::kThreads), smem, stream, a, b, g);
+    KGE_CUDA(err);
 }
 template <class TOut>
 void launch_product(int tile_m, const CUtensorMap& a, const CUtensorMap& b, const rows8::ProductArgs& g, cudaStream_t stream) {
     if (tile_m == 16) launch_product<16, TOut>(a, b, g, stream);
     else if (tile_m == 32) launch_product<32, TOut>(a, b, g, stream);
     else if (tile_m == 64) launch_product<64, TOut>(a, b, g, stream);
-    else launch_product<128, TOut>(a, b, g, stream);
+    else if (tile_m == 128) launch_product<128, TOut>(a, b, g, stream);
+    else launch_product<256, TOut>(a, b, g, stream);
 }
 
 }  // namespace
@@ -273,7 +278,7 @@ void product8(const uint8_t* a_values, const uint8_t* a_exponents, size_t m, con
         need(aligned_to(workspace, 256), "kge_op_product8: the workspace is not aligned to 256 bytes");
     }
     const CUtensorMap a = rows_map(a_values, m, k, p.tile_m), b = rows_map(b_values, n, k, rows8::kTileN);
-    rows8::ProductArgs g{a_exponents, b_exponents, out, out_row_stride, 0, (int)m, (int)n, p.blocks, (p.blocks + 3) / 4, p.n_tiles, p.m_tiles, p.splits};
+    rows8::ProductArgs g{a_exponents, b_exponents, out, out_row_stride, 0, (int)m, (int)n, p.blocks, (p.blocks + 3) / 4, p.n_tiles, p.m_tiles, p.splits, p.chunk};
     if (p.splits > 1) {
         g.out = workspace;
         g.out_stride = (long long)n;
@@ -281,8 +286,9 @@ void product8(const uint8_t* a_values, const uint8_t* a_exponents, size_t m, con
         launch_product<float>(p.tile_m, a, b, g, stream);
         with_type(out_type, [&](auto t) {
             using T = decltype(t);
-            rows8::k_add_splits<T><<<grid_of((m * n + 255) / 256, what), 256, 0, stream>>>(static_cast<const float*>(workspace), g.split_stride, p.splits, (int)m, (int)n,
-                                                                                   static_cast<T*>(out), out_row_stride);
+            const cudaError_t err = launch_dependent(rows8::k_add_splits<T>, dim3(grid_of((m * n + 255) / 256, what)), dim3(256), 0, stream, static_cast<const float*>(workspace),
+                                                     g.split_stride, p.splits, (int)m, (int)n, static_cast<T*>(out), out_row_stride);
+            KGE_CUDA(err);
         });
     } else {
         with_type(out_type, [&](auto t) { launch_product<decltype(t)>(p.tile_m, a, b, g, stream); });

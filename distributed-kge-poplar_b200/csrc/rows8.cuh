@@ -311,6 +311,21 @@ struct ProductArgs {
     long long split_stride;
     int m, n, blocks, groups;
     int n_tiles, m_tiles, splits;
+    int chunk;  // tiles of n that are gone through for all of m before the next ones
+};
+
+// A block's w-th tile.  Tiles that are worked on at the same time lie side by side along the rows of `out`, so that its memory is
+// written in long pieces (4096 x 62 500 bf16 results of 128-wide rows: ORDER1 us, with neighbours one above the other 294), in
+// chunks whose part of the table stays in L2 until all of m has met it.
+struct TilePlace {
+    int mt, nt, split;
+    __device__ __forceinline__ TilePlace(const ProductArgs& g, int w) {
+        const int tiles = g.m_tiles * g.n_tiles, i = w % tiles, whole = g.chunk * g.m_tiles;
+        split = w / tiles;
+        const int at = i / whole, r = i - at * whole, width = min(g.chunk, g.n_tiles - at * g.chunk);
+        mt = r / width;
+        nt = at * g.chunk + r - mt * width;
+    }
 };
 
 // The tensor core's two operands are the table (128 rows of b to the 128 lanes) and the queries (TM rows of a to as many
@@ -330,10 +345,12 @@ struct Tile {
     static constexpr int kStageBytes = kBBytes + kABytes + kGroupBytes * (1 + kAGroups);
     static constexpr int kTileBytes = (kStageBytes + 1023) / 1024 * 1024;  // the swizzle wants 1024-byte boundaries
     static constexpr int kStages = 200 * 1024 / kTileBytes < 10 ? 200 * 1024 / kTileBytes : 10;
-    static constexpr int kAccumulators = TM <= 128 ? 2 : 1;
-    static constexpr int kColumns = TM < 32 ? 32 : TM;
+    // Two accumulators, so that a tile is written out while the next one is summed.  Two of 256 columns leave no room for scales:
+    // they share 64, and the next tile begins once those are read, which are read first.
+    static constexpr bool kShare = TM > 128;
+    static constexpr int kNextColumns = kShare ? TM - 64 : TM < 32 ? 32 : TM;
     static constexpr int kScaleColumns = 4 * (1 + kAGroups);
-    static constexpr int kScale0 = kAccumulators * kColumns;
+    static constexpr int kScale0 = kNextColumns + (TM < 32 ? 32 : TM);
     static_assert(kScale0 + kStages * kScaleColumns <= kTmemColumns, "accumulators and scales share the tensor memory");
     static constexpr size_t smem() { return 1024 + (size_t)kStages * kTileBytes; }
 };
@@ -408,14 +425,14 @@ k_product8(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CU
     using L = Tile<TM>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    __shared__ uint64_t s_full[L::kStages], s_empty[L::kStages], s_done[L::kAccumulators], s_free[L::kAccumulators];
+    __shared__ uint64_t s_full[L::kStages], s_empty[L::kStages], s_done[2], s_free[2];  // s_free[0] alone where accumulators share columns
     __shared__ uint32_t s_tmem;
     __shared__ int s_gave_up;
     volatile int* const gave_up = &s_gave_up;
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < L::kStages; ++i) tc::mbar_init(&s_full[i], 1), tc::mbar_init(&s_empty[i], 1);
-        for (int i = 0; i < L::kAccumulators; ++i) tc::mbar_init(&s_done[i], 1), tc::mbar_init(&s_free[i], L::kEpilogueWarps);
+        for (int i = 0; i < 2; ++i) tc::mbar_init(&s_done[i], 1), tc::mbar_init(&s_free[i], L::kEpilogueWarps);
         tc::mbar_fence_init();
         s_gave_up = 0;
     }
@@ -423,6 +440,7 @@ k_product8(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CU
     tc::tc_fence_before();
     __syncthreads();
     tc::tc_fence_after();
+    grid_dependency_sync();
     const uint32_t tmem = s_tmem;
     const int n_work = g.n_tiles * g.m_tiles * g.splits;
 
@@ -431,7 +449,8 @@ k_product8(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CU
             int stage = 0;
             uint32_t parity = 1;  // the ring starts empty
             for (int w = blockIdx.x; w < n_work; w += gridDim.x) {
-                const int mt = w % g.m_tiles, nt = w / g.m_tiles % g.n_tiles, split = w / (g.m_tiles * g.n_tiles);
+                const TilePlace tile(g, w);
+                const int mt = tile.mt, nt = tile.nt, split = tile.split;
                 const int first = (int)((long long)g.blocks * split / g.splits), last = (int)((long long)g.blocks * (split + 1) / g.splits);
                 for (int kb = first; kb < last; ++kb) {
                     if (!wait(&s_empty[stage], parity, gave_up)) goto fetched;
@@ -459,7 +478,7 @@ k_product8(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CU
             for (int w = blockIdx.x; w < n_work; w += gridDim.x) {
                 const int split = w / (g.m_tiles * g.n_tiles);
                 const int first = (int)((long long)g.blocks * split / g.splits), last = (int)((long long)g.blocks * (split + 1) / g.splits);
-                if (!wait(&s_free[slot], slot_parity, gave_up)) goto multiplied;
+                if (!wait(&s_free[L::kShare ? 0 : slot], slot_parity, gave_up)) goto multiplied;
                 tc::tc_fence_after();
                 for (int kb = first; kb < last; ++kb) {
                     if (!wait(&s_full[stage], parity, gave_up)) goto multiplied;
@@ -472,12 +491,13 @@ k_product8(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CU
                     const uint32_t idesc = scaled_idesc(kTileN, TM, kb & 3);
 #pragma unroll
                     for (int q = 0; q < 4; ++q)  // 32 values of k each, 32 bytes further
-                        mma_scaled(tmem + slot * L::kColumns, b_desc + 2 * q, a_desc + 2 * q, idesc, scales, scales + 4, kb > first || q > 0);
+                        mma_scaled(tmem + slot * L::kNextColumns, b_desc + 2 * q, a_desc + 2 * q, idesc, scales, scales + 4, kb > first || q > 0);
                     tc::umma_commit(&s_empty[stage]);
                     if (++stage == L::kStages) stage = 0, parity ^= 1;
                 }
                 tc::umma_commit(&s_done[slot]);
-                if (++slot == L::kAccumulators) slot = 0, slot_parity ^= 1;
+                slot ^= 1;
+                if (L::kShare || slot == 0) slot_parity ^= 1;
             }
         multiplied:;
         }
@@ -487,23 +507,32 @@ k_product8(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CU
         int slot = 0;
         uint32_t parity = 0;
         for (int w = blockIdx.x; w < n_work; w += gridDim.x) {
-            const int mt = w % g.m_tiles, nt = w / g.m_tiles % g.n_tiles, split = w / (g.m_tiles * g.n_tiles);
+            const TilePlace tile(g, w);
+            const int mt = tile.mt, nt = tile.nt, split = tile.split;
             if (!wait(&s_done[slot], parity, gave_up)) break;
             tc::tc_fence_after();
             const int n = nt * kTileN + quad * 32 + lane, m0 = mt * TM + column0;
             TOut* const out = static_cast<TOut*>(g.out) + (size_t)split * g.split_stride + (long long)m0 * g.out_stride + n;
-#pragma unroll
-            for (int c = 0; c < L::kWarpColumns; c += 32) {
+            // of shared columns the warps that read them read them first: the last 64 of slot 0, the first 64 of slot 1
+            const int first = L::kShare && slot == 0 && column0 > 0 ? 64 : 0;
+            const auto release = [&] {
+                tc::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&s_free[L::kShare ? 0 : slot]);
+            };
+            if (L::kShare && (slot == 0) == (column0 == 0)) release();  // this warp reads none of them
+#pragma unroll 1
+            for (int i = 0; i < L::kWarpColumns; i += 32) {
+                const int c = i ^ first;
                 uint32_t acc[32];
-                tc::tmem_ld32(tmem + slot * L::kColumns + column0 + c + ((uint32_t)(quad * 32) << 16), acc);
+                tc::tmem_ld32(tmem + slot * L::kNextColumns + column0 + c + ((uint32_t)(quad * 32) << 16), acc);
+                if (L::kShare ? i == 32 && (slot == 0) != (column0 == 0) : i + 32 >= L::kWarpColumns) release();
                 constexpr int kRows = L::kWarpColumns < 32 ? L::kWarpColumns : 32;
                 const int rows = min(kRows, g.m - m0 - c);
                 store_columns<kRows>(out + (long long)c * g.out_stride, g.out_stride, acc, n < g.n ? rows : 0);
             }
-            tc::tc_fence_before();
-            __syncwarp();
-            if (lane == 0) tc::mbar_arrive(&s_free[slot]);
-            if (++slot == L::kAccumulators) slot = 0, parity ^= 1;
+            slot ^= 1;
+            if (slot == 0) parity ^= 1;
         }
     }
     tc::tc_fence_before();
@@ -522,6 +551,7 @@ k_product8(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CU
 template <class TOut>
 static __global__ void __launch_bounds__(256) k_add_splits(const float* __restrict__ partial, long long split_stride, int splits, int m, int n,
                                                            TOut* __restrict__ out, long long out_stride) {
+    grid_dependency_sync();
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
     if (i >= (long long)m * n) return;
     float sum = partial[i];
