@@ -2,14 +2,15 @@
 //
 //   m = beta_m m + (1 - beta_m) g,  v = beta_v v + (1 - beta_v) g^2,  p = p decay - step_size m / (sqrt(v) correction + epsilon)
 //
-// A warp takes a block of 128 values, 4 to a lane, in one pass: the block's largest new moments are known after one reduction
-// across the warp, before anything is written.
+// One pass: a block's largest new moments are known after one reduction across its lanes, before they are written.
 #pragma once
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+
+#include "pdl.cuh"
 
 namespace kge {
 namespace adamw {
@@ -26,7 +27,7 @@ __host__ __device__ __forceinline__ uint32_t mix(uint32_t x) {
 }
 
 struct Params {
-    float beta_m, one_minus_beta_m, beta_v, one_minus_beta_v, epsilon, grad_scale;
+    float beta_m, one_minus_beta_m, beta_v, one_minus_beta_v, epsilon;  // one_minus_beta times the gradients' scale, or its square
     float decay, step_size, correction;
     uint32_t key;
     const float* schedule;
@@ -36,8 +37,8 @@ struct Tensor {
     void* param;
     const void* grad;
     unsigned long long size;
-    unsigned long long first_block;  // of its moments
-    uint32_t blocks_end;             // blocks of this launch before the next tensor's (all tensors so far)
+    unsigned long long first;  // of its moments
+    uint32_t units_end;        // units of this launch (128 values, of 8-bit moments 512) before the next tensor's
     uint32_t aligned;                // 1: the vectors of both arrays are aligned
 };
 
@@ -47,55 +48,42 @@ struct Table {
     int n;
 };
 
-__device__ __forceinline__ float rounded_stochastically(float x, uint32_t r16) {  // to bf16, toward zero or away from it
-    const uint32_t b = __float_as_uint(x);
-    if ((b & 0x7f800000u) == 0x7f800000u) return __bfloat162float(__float2bfloat16_rn(x));  // stays infinite, or NaN
-    return __uint_as_float((b + r16) & 0xffff0000u);
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
 }
+// To bf16, toward zero or away from it, as an fp32.  An infinity stays one; a NaN's bits would run over.
+__device__ __forceinline__ float rounded_stochastically(float x, uint32_t r16) { return __uint_as_float((__float_as_uint(x) + r16) & 0xffff0000u); }
 
-// The codes of a block: TOP = 255 without a sign, 127 with one.
+// The codes of a block: TOP = 255 without a sign, 127 with one.  They are kept short: at 60 integer instructions a value a step in 8
+// bits was bound by them at three times the time that its bytes take.
 template <int TOP>
 __device__ __forceinline__ int block_exponent(uint32_t largest) {
     if (largest >= 0x7f800000u) return 255;
     return max((int)((largest + 0xfffffu) >> 23), TOP == 255 ? 33 : 16);
 }
+// What a code in units of 2^20 is added to, to be its value's bits.
 template <int TOP>
-__device__ __forceinline__ uint32_t encode(float x, int exponent, uint32_t r16) {
-    const uint32_t b = __float_as_uint(x), magnitude = b & 0x7fffffffu;
-    const int step = (int)((magnitude + (r16 << 4)) >> 20) - (8 * exponent + 7 - TOP);
-    int code = min(max(step, TOP == 255 && magnitude > 0 ? 1 : 0), TOP);
-    if (TOP == 127 && (b >> 31) && code > 0) code |= 128;
-    return (uint32_t)code;
+__device__ __forceinline__ uint32_t code_base(int exponent) { return (uint32_t)(8 * exponent + 7 - TOP) << 20; }
+template <int TOP>
+__device__ __forceinline__ float decode(uint32_t byte, uint32_t base) {
+    uint32_t bits = (byte << 20) + base;
+    if (TOP == 127) bits += (byte >> 7) * 0x78000000u;  // the sign from bit 27 to bit 31
+    return (byte & (uint32_t)TOP) ? __uint_as_float(bits) : 0.f;
 }
+// The code of a value of a finite block; none is above TOP, since the block's exponent is that of its largest value rounded up.
 template <int TOP>
-__device__ __forceinline__ float decode(uint32_t code, int exponent) {
-    if (exponent == 255) return __uint_as_float(0x7fc00000u);
-    const uint32_t c = code & (uint32_t)TOP;
-    const uint32_t magnitude = c ? (uint32_t)((int)c + (8 * exponent + 7 - TOP)) << 20 : 0u;
-    return __uint_as_float(magnitude | (TOP == 127 ? (code & 128u) << 24 : 0u));
+__device__ __forceinline__ uint32_t encode(float x, uint32_t base, uint32_t r16) {
+    const uint32_t b = __float_as_uint(x), magnitude = TOP == 127 ? b & 0x7fffffffu : b;
+    const int least = TOP == 255 ? (int)(min(magnitude, 1u) << 20) : 0;
+    const uint32_t code = (uint32_t)max((int)(r16 * 16u + (magnitude - base)), least) >> 20;
+    return TOP == 127 ? code | (b >> 24 & 128u) : code;
+}
+__device__ __forceinline__ uint32_t four_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 
-__device__ __forceinline__ void load_values(const float* p, float (&v)[4]) {
-    const float4 t = *reinterpret_cast<const float4*>(p);
-    v[0] = t.x, v[1] = t.y, v[2] = t.z, v[3] = t.w;
-}
-__device__ __forceinline__ void load_values(const __nv_bfloat16* p, float (&v)[4]) {
-    const uint2 t = *reinterpret_cast<const uint2*>(p);
-    v[0] = __uint_as_float(t.x << 16), v[1] = __uint_as_float(t.x & 0xffff0000u);
-    v[2] = __uint_as_float(t.y << 16), v[3] = __uint_as_float(t.y & 0xffff0000u);
-}
-__device__ __forceinline__ void load_values(const __half* p, float (&v)[4]) {
-    const uint2 t = *reinterpret_cast<const uint2*>(p);
-    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&t.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&t.y));
-    v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
-}
-__device__ __forceinline__ void store_values(float* p, const float (&v)[4]) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
-__device__ __forceinline__ void store_values(__nv_bfloat16* p, const float (&v)[4]) {  // exact: the values are bf16 already
-    uint2 t;
-    t.x = __float_as_uint(v[0]) >> 16 | (__float_as_uint(v[1]) & 0xffff0000u);
-    t.y = __float_as_uint(v[2]) >> 16 | (__float_as_uint(v[3]) & 0xffff0000u);
-    *reinterpret_cast<uint2*>(p) = t;
-}
 __device__ __forceinline__ float value(const float* p) { return *p; }
 __device__ __forceinline__ float value(const __half* p) { return __half2float(*p); }
 __device__ __forceinline__ float value(const __nv_bfloat16* p) { return __bfloat162float(*p); }
@@ -103,88 +91,270 @@ __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
 constexpr int kThreads = 256;
+constexpr int kBlocksPerWarp = 2;  // fetched together
 
-template <class TP, class TG, int BITS, int MAX>
-static __global__ void __launch_bounds__(kThreads) k_adamw(const __grid_constant__ Table<MAX> table, Params a, void* adam_m, void* adam_v,
-                                                           uint8_t* __restrict__ m_exponent, uint8_t* __restrict__ v_exponent) {
-    constexpr bool kBf16 = sizeof(TP) == 2;
-    const uint32_t unit = blockIdx.x * (kThreads / 32) + threadIdx.x / 32;
-    if (unit >= table.t[table.n - 1].blocks_end) return;
-    int lo = 0, hi = table.n - 1;  // the first tensor whose end is past this block
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (table.t[mid].blocks_end > unit) hi = mid;
-        else lo = mid + 1;
+__device__ __forceinline__ float quick_sqrt(float x) {
+    float y;
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float quick_reciprocal(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Four values of a lane as they lie in memory.
+template <class T>
+struct Quad;
+template <>
+struct Quad<float> {
+    float4 raw;
+    __device__ __forceinline__ void load(const float* p) { raw = *reinterpret_cast<const float4*>(p); }
+    __device__ __forceinline__ void floats(float (&v)[4]) const { v[0] = raw.x, v[1] = raw.y, v[2] = raw.z, v[3] = raw.w; }
+    __device__ __forceinline__ void set(const float (&v)[4]) { raw = make_float4(v[0], v[1], v[2], v[3]); }
+};
+template <class T>
+struct HalfQuad {
+    uint2 raw;
+    __device__ __forceinline__ void load(const T* p) { raw = *reinterpret_cast<const uint2*>(p); }
+};
+template <>
+struct Quad<__nv_bfloat16> : HalfQuad<__nv_bfloat16> {
+    __device__ __forceinline__ void floats(float (&v)[4]) const {
+        v[0] = __uint_as_float(raw.x << 16), v[1] = __uint_as_float(raw.x & 0xffff0000u), v[2] = __uint_as_float(raw.y << 16), v[3] = __uint_as_float(raw.y & 0xffff0000u);
     }
-    const Tensor& t = table.t[lo];
-    const uint32_t local = unit - (lo > 0 ? table.t[lo - 1].blocks_end : 0u);
-    const int lane = threadIdx.x & 31;
-    const unsigned long long i0 = (unsigned long long)local * kBlock + lane * 4;           // in the tensor
-    const unsigned long long block = t.first_block + local, at = block * kBlock + lane * 4;  // in the moments
-    float decay = a.decay, step_size = a.step_size, correction = a.correction;
-    uint32_t key = a.key;
-    if (a.schedule) decay = a.schedule[0], step_size = a.schedule[1], correction = a.schedule[2], key = __float_as_uint(a.schedule[3]);
+    __device__ __forceinline__ void set(const float (&v)[4]) {  // of values that are bf16
+        raw.x = __byte_perm(__float_as_uint(v[0]), __float_as_uint(v[1]), 0x7632);
+        raw.y = __byte_perm(__float_as_uint(v[2]), __float_as_uint(v[3]), 0x7632);
+    }
+};
+template <>
+struct Quad<__half> : HalfQuad<__half> {
+    __device__ __forceinline__ void floats(float (&v)[4]) const {
+        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&raw.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&raw.y));
+        v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
+    }
+    __device__ __forceinline__ void set(const float (&v)[4]) {
+        const __half2 a = __floats2half2_rn(v[0], v[1]), b = __floats2half2_rn(v[2], v[3]);
+        raw.x = *reinterpret_cast<const uint32_t*>(&a), raw.y = *reinterpret_cast<const uint32_t*>(&b);
+    }
+};
+// The lane's values of a tensor that begin `live` before its end, zeros past it.
+template <class T>
+__device__ __forceinline__ void load_quad(Quad<T>& q, const T* p, int live, bool whole) {
+    if (whole) {
+        q.load(p);
+        return;
+    }
+    float v[4] = {};
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (j < live) v[j] = value(p + j);
+    q.set(v);
+}
 
+// The tensor of a launch's block: the first whose end is past it.  All lanes of a warp look at once.
+template <int MAX>
+__device__ __forceinline__ int tensor_of(const Table<MAX>& table, uint32_t unit) {
+    const int lane = threadIdx.x & 31;
+    int at = 0;
+    for (int base = 0; base < table.n; base += 32) {
+        const bool before = base + lane < table.n && table.t[base + lane].units_end <= unit;
+        const int n = __popc(__ballot_sync(~0u, before));
+        at += n;
+        if (n < 32) break;
+    }
+    return at;
+}
+
+struct Step {
+    float beta_m, one_minus_beta_m, beta_v, one_minus_beta_v, epsilon, decay, step_size, correction;
+    uint32_t key;
+    __device__ __forceinline__ Step(const Params& a)
+        : beta_m(a.beta_m), one_minus_beta_m(a.one_minus_beta_m), beta_v(a.beta_v), one_minus_beta_v(a.one_minus_beta_v), epsilon(a.epsilon), decay(a.decay),
+          step_size(a.step_size), correction(a.correction), key(a.key) {
+        if (a.schedule) decay = a.schedule[0], step_size = a.schedule[1], correction = a.schedule[2], key = __float_as_uint(a.schedule[3]);
+    }
+    // Root and reciprocal to 2^-22: the step that they scale is a thousandth of the parameter, whose own rounding is 2^-24 or more.
+    __device__ __forceinline__ void take(float& p, float g, float& m, float& v) const {
+        m = fmaf(beta_m, m, one_minus_beta_m * g);
+        v = fmaf(beta_v, v, one_minus_beta_v * g * g);
+        p = fmaf(p, decay, -step_size * m * quick_reciprocal(fmaf(quick_sqrt(v), correction, epsilon)));
+    }
+    // What is mixed for the values from a position (a multiple of 4) on.
+    __device__ __forceinline__ uint32_t mixed(unsigned long long at) const { return (uint32_t)at * 0x9E3779B9u + (uint32_t)(at >> 32) * 0x6A09E667u + key; }
+};
+// Bits 8 to 23 of a draw.
+__device__ __forceinline__ uint32_t middle(uint32_t draw) { return __byte_perm(draw, 0, 0x4421); }
+template <int N>
+__device__ __forceinline__ void round_all(float (&p)[N], const uint32_t (&draw)[N]) {
+    float sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) sum += fabsf(p[j]);
+    const bool finite = sum < INFINITY;  // else one by one: a NaN's bits would run over
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const float rounded = rounded_stochastically(p[j], middle(draw[j]));
+        p[j] = finite || p[j] == p[j] ? rounded : __uint_as_float(0x7fc00000u);
+    }
+}
+
+// Moments in fp32: a warp takes 128 values at a time, four to a lane, and two such units, fetched together.
+template <class TP, class TG, int MAX>
+static __global__ void __launch_bounds__(kThreads, 3) k_adamw32(const __grid_constant__ Table<MAX> table, Params a, float* __restrict__ adam_m, float* __restrict__ adam_v) {
+    constexpr int kUnits = kBlocksPerWarp;
+    grid_dependency_sync();
+    const uint32_t n_units = table.t[table.n - 1].units_end;
+    const uint32_t first = (blockIdx.x * (kThreads / 32) + threadIdx.x / 32) * kUnits;
+    if (first >= n_units) return;
+    const int lane = threadIdx.x & 31;
+    const Step step(a);
+    Quad<TP> p_raw[kUnits];
+    Quad<TG> g_raw[kUnits];
+    float4 m_raw[kUnits], v_raw[kUnits];
+    TP* param[kUnits];
+    unsigned long long at[kUnits];
+    int live[kUnits];
+    bool whole[kUnits];
+    int index = tensor_of(table, first);
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+        const uint32_t unit = min(first + u, n_units - 1);  // the last is read, but not written, again
+        while (table.t[index].units_end <= unit) ++index;
+        const Tensor& t = table.t[index];
+        const unsigned long long i0 = (unsigned long long)(unit - (index > 0 ? table.t[index - 1].units_end : 0u)) * kBlock + lane * 4;  // in the tensor
+        at[u] = t.first + i0;  // in the moments
+        live[u] = i0 >= t.size ? 0 : t.size - i0 >= 4 ? 4 : (int)(t.size - i0);
+        whole[u] = live[u] == 4 && t.aligned;
+        param[u] = static_cast<TP*>(t.param) + i0;
+        load_quad(p_raw[u], static_cast<const TP*>(param[u]), live[u], whole[u]);
+        load_quad(g_raw[u], static_cast<const TG*>(t.grad) + i0, live[u], whole[u]);
+        m_raw[u] = *reinterpret_cast<const float4*>(adam_m + at[u]);
+        v_raw[u] = *reinterpret_cast<const float4*>(adam_v + at[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+        if (first + u >= n_units) return;
+        float p[4], g[4], m[4] = {m_raw[u].x, m_raw[u].y, m_raw[u].z, m_raw[u].w}, v[4] = {v_raw[u].x, v_raw[u].y, v_raw[u].z, v_raw[u].w};
+        p_raw[u].floats(p);
+        g_raw[u].floats(g);
+        // past the tensor's end gradient and moments are 0, and stay so
+#pragma unroll
+        for (int j = 0; j < 4; ++j) step.take(p[j], g[j], m[j], v[j]);
+        if constexpr (sizeof(TP) == 2) {
+            uint32_t draw[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) draw[j] = mix(step.mixed(at[u]) + (uint32_t)j * 0x9E3779B9u);
+            round_all(p, draw);
+        }
+        if (whole[u]) {
+            Quad<TP> out;
+            out.set(p);
+            *reinterpret_cast<decltype(out.raw)*>(param[u]) = out.raw;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (j < live[u]) put(param[u] + j, p[j]);
+        }
+        *reinterpret_cast<float4*>(adam_m + at[u]) = make_float4(m[0], m[1], m[2], m[3]);
+        *reinterpret_cast<float4*>(adam_v + at[u]) = make_float4(v[0], v[1], v[2], v[3]);
+    }
+}
+
+// Moments in 8 bits: a warp takes four blocks of 128 values, eight lanes and 16 values a lane each, so that what a lane does but once
+// (finding its place, the exponents) is spread over 16 values: with four a lane a step took 92 instructions a value.
+constexpr int kLaneValues = 16;
+template <class TP, class TG, int MAX>
+static __global__ void __launch_bounds__(kThreads, 2) k_adamw8(const __grid_constant__ Table<MAX> table, Params a, uint8_t* __restrict__ adam_m, uint8_t* __restrict__ adam_v,
+                                                               uint8_t* __restrict__ m_exponent, uint8_t* __restrict__ v_exponent) {
+    constexpr int N = kLaneValues;
+    grid_dependency_sync();
+    const uint32_t unit = blockIdx.x * (kThreads / 32) + threadIdx.x / 32;
+    if (unit >= table.t[table.n - 1].units_end) return;
+    const int lane = threadIdx.x & 31, index = tensor_of(table, unit);
+    const Tensor& t = table.t[index];
+    const unsigned long long i0 = (unsigned long long)(unit - (index > 0 ? table.t[index - 1].units_end : 0u)) * (4 * kBlock) + lane * N;  // in the tensor
+    const bool here = (i0 & ~(unsigned long long)(kBlock - 1)) < t.size;  // the block is this tensor's, for all of its lanes
+    const unsigned long long at = t.first + i0, block = at / kBlock;      // in the moments
+    const int live = i0 >= t.size ? 0 : t.size - i0 >= N ? N : (int)(t.size - i0);
+    const bool whole = live == N && t.aligned;
     TP* const param = static_cast<TP*>(t.param) + i0;
     const TG* const grad = static_cast<const TG*>(t.grad) + i0;
-    const int live = i0 >= t.size ? 0 : t.size - i0 >= 4 ? 4 : (int)(t.size - i0);
-    const bool whole = live == 4 && t.aligned;
-    float p[4] = {}, g[4] = {}, m[4], v[4];
-    if (whole) {
-        load_values(param, p);
-        load_values(grad, g);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (j < live) p[j] = value(param + j), g[j] = value(grad + j);
+    Quad<TP> p_raw[N / 4];
+    Quad<TG> g_raw[N / 4];
+    uint4 m_raw = make_uint4(0, 0, 0, 0), v_raw = m_raw;
+    int em = 16, ev = 33;
+    if (here) {
+        m_raw = *reinterpret_cast<const uint4*>(adam_m + at);
+        v_raw = *reinterpret_cast<const uint4*>(adam_v + at);
+        em = m_exponent[block], ev = v_exponent[block];
     }
-    if (BITS == 32) {
-        load_values(static_cast<const float*>(adam_m) + at, m);
-        load_values(static_cast<const float*>(adam_v) + at, v);
-    } else {
-        const uint32_t cm = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(adam_m) + at);
-        const uint32_t cv = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(adam_v) + at);
-        const int em = m_exponent[block], ev = v_exponent[block];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) m[j] = decode<127>(cm >> (8 * j) & 255u, em), v[j] = decode<255>(cv >> (8 * j) & 255u, ev);
-    }
-    uint32_t draw[4];
-    const uint32_t base = (uint32_t)at * 0x9E3779B9u + (uint32_t)(at >> 32) * 0x6A09E667u + key;
-    uint32_t largest_m = 0, largest_v = 0;
+    for (int q = 0; q < N / 4; ++q) load_quad(p_raw[q], static_cast<const TP*>(param) + 4 * q, live - 4 * q, whole), load_quad(g_raw[q], grad + 4 * q, live - 4 * q, whole);
+    const Step step(a);
+    float m[N], v[N], largest_m = 0.f, largest_v = 0.f;
+    uint32_t draw[N];
+    {
+        const uint32_t base_m = code_base<127>(em), base_v = code_base<255>(ev);
+        const uint32_t mw[4] = {m_raw.x, m_raw.y, m_raw.z, m_raw.w}, vw[4] = {v_raw.x, v_raw.y, v_raw.z, v_raw.w};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const float gj = g[j] * a.grad_scale;
-        m[j] = fmaf(a.beta_m, m[j], a.one_minus_beta_m * gj);
-        v[j] = fmaf(a.beta_v, v[j], a.one_minus_beta_v * gj * gj);
-        p[j] = p[j] * decay - step_size * m[j] / (sqrtf(v[j]) * correction + a.epsilon);
-        if (BITS == 8 || kBf16) draw[j] = mix(base + (uint32_t)j * 0x9E3779B9u);
-        if (kBf16) p[j] = rounded_stochastically(p[j], draw[j] >> 8 & 0xffffu);
-        if (j >= live) m[j] = v[j] = 0.f;  // the block's rest stays zero
-        largest_m = max(largest_m, __float_as_uint(m[j]) & 0x7fffffffu);
-        largest_v = max(largest_v, __float_as_uint(v[j]) & 0x7fffffffu);
-    }
-    if (whole) {
-        store_values(param, p);
-    } else {
+        for (int j = 0; j < N; ++j) {
+            m[j] = decode<127>(__byte_perm(mw[j / 4], 0, 0x4440 + j % 4), base_m);
+            v[j] = decode<255>(__byte_perm(vw[j / 4], 0, 0x4440 + j % 4), base_v);
+        }
+        if (em == 255 || ev == 255) {
+            const float nan = __uint_as_float(0x7fc00000u);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (j < live) put(param + j, p[j]);
+            for (int j = 0; j < N; ++j) m[j] = em == 255 ? nan : m[j], v[j] = ev == 255 ? nan : v[j];
+        }
     }
-    if (BITS == 32) {
-        store_values(static_cast<float*>(adam_m) + at, m);
-        store_values(static_cast<float*>(adam_v) + at, v);
-    } else {
-        const int em = block_exponent<127>(__reduce_max_sync(~0u, largest_m)), ev = block_exponent<255>(__reduce_max_sync(~0u, largest_v));
-        uint32_t cm = 0, cv = 0;
+    const uint32_t base = step.mixed(at);
+#pragma unroll
+    for (int q = 0; q < N / 4; ++q) {
+        float p[4], g[4];
+        uint32_t d[4];
+        p_raw[q].floats(p);
+        g_raw[q].floats(g);
+        // past the tensor's end gradient and moments are 0, and stay so
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            cm |= encode<127>(m[j], em, draw[j] & 0xffffu) << (8 * j);
-            cv |= encode<255>(v[j], ev, draw[j] >> 16) << (8 * j);
+            step.take(p[j], g[j], m[4 * q + j], v[4 * q + j]);
+            d[j] = draw[4 * q + j] = mix(base + (uint32_t)(4 * q + j) * 0x9E3779B9u);
+            largest_m = max_or_nan(largest_m, fabsf(m[4 * q + j]));
+            largest_v = max_or_nan(largest_v, v[4 * q + j]);
         }
-        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(adam_m) + at) = cm;
-        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(adam_v) + at) = cv;
-        if (lane == 0) m_exponent[block] = (uint8_t)em, v_exponent[block] = (uint8_t)ev;
+        if constexpr (sizeof(TP) == 2) round_all(p, d);
+        if (whole) {
+            Quad<TP> out;
+            out.set(p);
+            *reinterpret_cast<decltype(out.raw)*>(param + 4 * q) = out.raw;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (4 * q + j < live) put(param + 4 * q + j, p[j]);
+        }
     }
+    uint32_t top_m = __float_as_uint(largest_m), top_v = __float_as_uint(largest_v);
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) top_m = max(top_m, __shfl_xor_sync(~0u, top_m, o)), top_v = max(top_v, __shfl_xor_sync(~0u, top_v, o));
+    if (!here) return;
+    const int new_em = block_exponent<127>(top_m), new_ev = block_exponent<255>(top_v);
+    const uint32_t base_m = code_base<127>(new_em), base_v = code_base<255>(new_ev);
+    uint32_t mw[4], vw[4];
+#pragma unroll
+    for (int q = 0; q < N / 4; ++q) {
+        uint32_t c[4], d[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            c[j] = encode<127>(m[4 * q + j], base_m, draw[4 * q + j] & 0xffffu);
+            d[j] = encode<255>(v[4 * q + j], base_v, draw[4 * q + j] >> 16);
+        }
+        mw[q] = four_bytes(c[0], c[1], c[2], c[3]), vw[q] = four_bytes(d[0], d[1], d[2], d[3]);
+    }
+    *reinterpret_cast<uint4*>(adam_m + at) = make_uint4(mw[0], mw[1], mw[2], mw[3]);
+    *reinterpret_cast<uint4*>(adam_v + at) = make_uint4(vw[0], vw[1], vw[2], vw[3]);
+    if ((lane & 7) == 0) m_exponent[block] = (uint8_t)new_em, v_exponent[block] = (uint8_t)new_ev;
 }
 
 static __global__ void __launch_bounds__(kThreads) k_moments(const uint8_t* __restrict__ adam_m, const uint8_t* __restrict__ m_exponent,
@@ -195,11 +365,19 @@ static __global__ void __launch_bounds__(kThreads) k_moments(const uint8_t* __re
     const size_t at = block * kBlock + (threadIdx.x & 31) * 4;
     const uint32_t cm = *reinterpret_cast<const uint32_t*>(adam_m + at), cv = *reinterpret_cast<const uint32_t*>(adam_v + at);
     const int em = m_exponent[block], ev = v_exponent[block];
+    const uint32_t base_m = code_base<127>(em), base_v = code_base<255>(ev);
+    const float nan = __uint_as_float(0x7fc00000u);
     float m[4], v[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) m[j] = decode<127>(cm >> (8 * j) & 255u, em), v[j] = decode<255>(cv >> (8 * j) & 255u, ev);
-    store_values(m_out + at, m);
-    store_values(v_out + at, v);
+    for (int j = 0; j < 4; ++j) {
+        m[j] = em == 255 ? nan : decode<127>(cm >> (8 * j) & 255u, base_m);
+        v[j] = ev == 255 ? nan : decode<255>(cv >> (8 * j) & 255u, base_v);
+    }
+    Quad<__nv_bfloat16> out;
+    out.set(m);
+    *reinterpret_cast<uint2*>(m_out + at) = out.raw;
+    out.set(v);
+    *reinterpret_cast<uint2*>(v_out + at) = out.raw;
 }
 
 }  // namespace adamw

@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "adamw.cuh"
 #include "log_probs.cuh"
@@ -217,24 +218,46 @@ ProductPlan product_plan(size_t m, size_t n, size_t k) {
     return p;
 }
 
-CUtensorMap rows_map(const uint8_t* values, size_t rows, size_t cols, int box_rows) {
+CUtensorMap encoded_map(CUtensorMapDataType type, const void* base, cuuint64_t cols, cuuint64_t rows, cuuint64_t stride_bytes, cuuint32_t box_cols, cuuint32_t box_rows,
+                        CUtensorMapSwizzle swizzle) {
     tc::EncodeTiledFn encode = tc::encode_tiled_fn();
     if (!encode) fail(KGE_RUNTIME_ERROR, "kge_op_product8: the driver has no cuTensorMapEncodeTiled");
     CUtensorMap map;
-    const cuuint64_t dims[2] = {cols, rows}, strides[1] = {rows8::value_stride(cols)};
-    const cuuint32_t box[2] = {rows8::kBlock, (cuuint32_t)box_rows}, step[2] = {1, 1};
-    if (encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(values), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    const cuuint64_t dims[2] = {cols, rows}, strides[1] = {stride_bytes};
+    const cuuint32_t box[2] = {box_cols, box_rows}, step[2] = {1, 1};
+    if (encode(&map, type, 2, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         fail(KGE_RUNTIME_ERROR, "kge_op_product8: a tensor map was refused");
     return map;
 }
+CUtensorMap rows_map(const uint8_t* values, size_t rows, size_t cols, int box_rows) {
+    return encoded_map(CU_TENSOR_MAP_DATA_TYPE_UINT8, values, cols, rows, rows8::value_stride(cols), rows8::kBlock, (cuuint32_t)box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+template <class T>
+constexpr CUtensorMapDataType map_type() {
+    return sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+}
 
 template <int TM, class TOut>
-void launch_product(const CUtensorMap& a, const CUtensorMap& b, const rows8::ProductArgs& g, cudaStream_t stream) {
-    constexpr size_t smem = rows8::Tile<TM>::smem();
-    allow_shared_memory<rows8::k_product8<TM, TOut>>(smem);
-    const int work = g.n_tiles * g.m_tiles * g.splits;
-    const cudaError_t err = launch_dependent(rows8::k_product8<TM, TOut>, dim3(std::min(work, kSmCount)), dim3(rows8::Tile<TM>::kThreads), smem, stream, a, b, g);
+void launch_product(const CUtensorMap& a, const CUtensorMap& b, rows8::ProductArgs g, cudaStream_t stream) {
+    using L = rows8::Tile<TM>;
+    CUtensorMap out = b;  // where results are stored directly, any map
+    const bool resident = g.blocks <= L::kMostResident && g.splits == 1 && g.m_tiles <= kSmCount;
+    g.stages = resident ? L::lone_stages(g.blocks) : L::kPairStages;
+    g.staged = TM >= 64 && resident && aligned_to(g.out, 16) && (g.m == 1 || g.out_stride * (long long)sizeof(TOut) % 16 == 0);
+    if (g.staged)
+        out = encoded_map(map_type<TOut>(), g.out, (cuuint64_t)g.n, (cuuint64_t)g.m, round_up((size_t)std::max<long long>(g.out_stride, g.n) * sizeof(TOut), 16),
+                          rows8::kBoxColumns<TOut>, rows8::kBoxRows<TOut>, sizeof(TOut) == 4 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B);
+    cudaError_t err;
+    if (resident) {
+        allow_shared_memory<rows8::k_product8<TM, TOut, true>>(L::smem());
+        const int grid = std::min(g.n_tiles, kSmCount / g.m_tiles) * g.m_tiles;
+        err = launch_dependent(rows8::k_product8<TM, TOut, true>, dim3(grid), dim3(L::kThreads), L::smem(), stream, a, b, out, g);
+    } else {
+        allow_shared_memory<rows8::k_product8<TM, TOut, false>>(L::smem());
+        const int work = g.n_tiles * g.m_tiles * g.splits;
+        err = launch_dependent(rows8::k_product8<TM, TOut, false>, dim3(std::min(work, kSmCount)), dim3(L::kThreads), L::smem(), stream, a, b, out, g);
+    }
     KGE_CUDA(err);
 }
 template <class TOut>
@@ -278,7 +301,7 @@ void product8(const uint8_t* a_values, const uint8_t* a_exponents, size_t m, con
         need(aligned_to(workspace, 256), "kge_op_product8: the workspace is not aligned to 256 bytes");
     }
     const CUtensorMap a = rows_map(a_values, m, k, p.tile_m), b = rows_map(b_values, n, k, rows8::kTileN);
-    rows8::ProductArgs g{a_exponents, b_exponents, out, out_row_stride, 0, (int)m, (int)n, p.blocks, (p.blocks + 3) / 4, p.n_tiles, p.m_tiles, p.splits, p.chunk};
+    rows8::ProductArgs g{a_exponents, b_exponents, out, out_row_stride, 0, (int)m, (int)n, p.blocks, (p.blocks + 3) / 4, p.n_tiles, p.m_tiles, p.splits, p.chunk, 0, 0};
     if (p.splits > 1) {
         g.out = workspace;
         g.out_stride = (long long)n;
@@ -310,20 +333,24 @@ bool product8_gave_up() {
 
 namespace {
 
-template <class TP, class TG, int BITS, int MAX>
+template <class TP, class TG, int MAX>
 void launch_adamw(const adamw::Table<adamw::kMaxTensors>& all, const adamw::Params& p, const kge_adamw_args& a, cudaStream_t stream) {
     adamw::Table<MAX> table;
     table.n = all.n;
     std::copy(all.t, all.t + all.n, table.t);
-    const uint32_t blocks = all.t[all.n - 1].blocks_end;
-    constexpr uint32_t per = adamw::kThreads / 32;
-    adamw::k_adamw<TP, TG, BITS, MAX><<<(blocks + per - 1) / per, adamw::kThreads, 0, stream>>>(table, p, a.adam_m, a.adam_v, a.m_exponent, a.v_exponent);
-    KGE_CUDA(cudaGetLastError());
+    const uint32_t per = adamw::kThreads / 32 * (a.state_bits == 8 ? 1 : adamw::kBlocksPerWarp), grid = (all.t[all.n - 1].units_end + per - 1) / per;
+    cudaError_t err;
+    if (a.state_bits == 8)
+        err = launch_dependent(adamw::k_adamw8<TP, TG, MAX>, dim3(grid), dim3(adamw::kThreads), 0, stream, table, p, static_cast<uint8_t*>(a.adam_m),
+                               static_cast<uint8_t*>(a.adam_v), a.m_exponent, a.v_exponent);
+    else
+        err = launch_dependent(adamw::k_adamw32<TP, TG, MAX>, dim3(grid), dim3(adamw::kThreads), 0, stream, table, p, static_cast<float*>(a.adam_m), static_cast<float*>(a.adam_v));
+    KGE_CUDA(err);
 }
-template <class TP, class TG, int BITS>
+template <class TP, class TG>
 void launch_adamw(const adamw::Table<adamw::kMaxTensors>& all, const adamw::Params& p, const kge_adamw_args& a, cudaStream_t stream) {
-    if (all.n <= 16) launch_adamw<TP, TG, BITS, 16>(all, p, a, stream);
-    else launch_adamw<TP, TG, BITS, adamw::kMaxTensors>(all, p, a, stream);
+    if (all.n <= 16) launch_adamw<TP, TG, 16>(all, p, a, stream);
+    else launch_adamw<TP, TG, adamw::kMaxTensors>(all, p, a, stream);
 }
 
 }  // namespace
@@ -334,11 +361,12 @@ void adamw_step(const kge_adamw_args& a, const kge_adamw_tensor* tensors, size_t
     const size_t param_bytes = a.param_type == KGE_F32 ? 4 : 2, grad_bytes = type_bytes(a.grad_type, what);
     if (a.state_bits != 8 && a.state_bits != 32) fail(KGE_INVALID_ARGUMENT, msg() << what << ": state_bits must be 8 or 32, not " << a.state_bits);
     need(n_tensors == 0 || tensors, "kge_op_adamw: null tensors");
-    const adamw::Params p{(float)a.beta_m, (float)(1. - a.beta_m), (float)a.beta_v, (float)(1. - a.beta_v), (float)a.epsilon, (float)a.grad_scale,
+    const adamw::Params p{(float)a.beta_m, (float)((1. - a.beta_m) * a.grad_scale), (float)a.beta_v, (float)((1. - a.beta_v) * a.grad_scale * a.grad_scale), (float)a.epsilon,
                           (float)a.decay, (float)a.step_size, (float)a.inv_sqrt_correction, a.key, a.schedule};
     adamw::Table<adamw::kMaxTensors> table;
     table.n = 0;
-    uint32_t blocks = 0;
+    uint32_t units = 0;
+    const size_t unit_values = adamw::kBlock * (a.state_bits == 8 ? 4 : 1);
     for (size_t i = 0; i < n_tensors; ++i) {
         const kge_adamw_tensor& t = tensors[i];
         if (!t.size) continue;
@@ -357,24 +385,21 @@ void adamw_step(const kge_adamw_args& a, const kge_adamw_tensor* tensors, size_t
         if (table.n == 0) return;
         with_type(a.grad_type, [&](auto g) {
             using TG = decltype(g);
-            if (a.param_type == KGE_F32) {
-                if (a.state_bits == 32) launch_adamw<float, TG, 32>(table, p, a, stream);
-                else launch_adamw<float, TG, 8>(table, p, a, stream);
-            } else {
-                if (a.state_bits == 32) launch_adamw<__nv_bfloat16, TG, 32>(table, p, a, stream);
-                else launch_adamw<__nv_bfloat16, TG, 8>(table, p, a, stream);
-            }
+            if (a.param_type == KGE_F32) launch_adamw<float, TG>(table, p, a, stream);
+            else launch_adamw<__nv_bfloat16, TG>(table, p, a, stream);
         });
         table.n = 0;
-        blocks = 0;
+        units = 0;
     };
     for (size_t i = 0; i < n_tensors; ++i) {
         const kge_adamw_tensor& t = tensors[i];
         if (!t.size) continue;
-        const uint32_t more = (uint32_t)((t.size + adamw::kBlock - 1) / adamw::kBlock);
-        if (table.n == adamw::kMaxTensors || more > 0x7fffffffu - blocks) flush();
-        blocks += more;
-        table.t[table.n++] = adamw::Tensor{t.param, t.grad, t.size, t.first / adamw::kBlock, blocks, aligned_to(t.param, 4 * param_bytes) && aligned_to(t.grad, 4 * grad_bytes)};
+        const uint32_t more = (uint32_t)((t.size + unit_values - 1) / unit_values);
+        if (table.n == adamw::kMaxTensors || more > 0x7fffffffu - units) flush();
+        units += more;
+        const size_t vector = a.state_bits == 8 ? 16 : 0;  // of 8-bit moments' lanes; else four values
+        table.t[table.n++] = adamw::Tensor{t.param, t.grad, t.size, t.first, units,
+                                           aligned_to(t.param, std::max(vector, 4 * param_bytes)) && aligned_to(t.grad, std::max(vector, 4 * grad_bytes))};
     }
     flush();
 }

@@ -312,20 +312,48 @@ struct ProductArgs {
     int m, n, blocks, groups;
     int n_tiles, m_tiles, splits;
     int chunk;  // tiles of n that are gone through for all of m before the next ones
+    int stages; // of the ring
+    int staged; // 1: `out` takes whole boxes of a tile's rows
 };
 
-// A block's w-th tile.  Tiles that are worked on at the same time lie side by side along the rows of `out`, so that its memory is
-// written in long pieces (4096 x 62 500 bf16 results of 128-wide rows: ORDER1 us, with neighbours one above the other 294), in
-// chunks whose part of the table stays in L2 until all of m has met it.
-struct TilePlace {
+// The tiles of a block, one after another.  Tiles that are worked on at the same time lie side by side along the rows of `out`, so
+// that its memory is written in long pieces (4096 x 62 500 bf16 results of 128-wide rows: 239 us, with neighbours one above the other
+// 294), in chunks whose part of the table stays in L2 until all of m has met it.  A block that keeps its rows of `a` goes along them.
+template <bool RESIDENT>
+struct Tiles {
+    int w, step, n_work, stride, run;
     int mt, nt, split;
-    __device__ __forceinline__ TilePlace(const ProductArgs& g, int w) {
-        const int tiles = g.m_tiles * g.n_tiles, i = w % tiles, whole = g.chunk * g.m_tiles;
-        split = w / tiles;
-        const int at = i / whole, r = i - at * whole, width = min(g.chunk, g.n_tiles - at * g.chunk);
-        mt = r / width;
-        nt = at * g.chunk + r - mt * width;
+    __device__ __forceinline__ Tiles(const ProductArgs& g) {
+        if (RESIDENT) {
+            mt = (int)blockIdx.x % g.m_tiles;
+            w = 0;
+            step = 1;
+            stride = (int)gridDim.x / g.m_tiles;
+            run = stride < 16 ? 4 : 1;  // where few blocks work on a row of `out`, each does four tiles side by side (292 -> 239 us)
+            n_work = (int)blockIdx.x < stride * g.m_tiles ? g.n_tiles : 0;
+            split = 0;
+        } else {
+            w = (int)blockIdx.x;
+            step = (int)gridDim.x;
+            n_work = g.n_tiles * g.m_tiles * g.splits;
+        }
     }
+    __device__ __forceinline__ bool here(const ProductArgs& g) {
+        if (RESIDENT) {
+            nt = (w / run * stride + (int)blockIdx.x / g.m_tiles) * run + w % run;
+            if (nt >= n_work) return false;
+        } else {
+            if (w >= n_work) return false;
+            const int tiles = g.m_tiles * g.n_tiles, i = w % tiles, whole = g.chunk * g.m_tiles;
+            split = w / tiles;
+            const int at = i / whole, r = i - at * whole, width = min(g.chunk, g.n_tiles - at * g.chunk);
+            mt = r / width;
+            nt = at * g.chunk + r - mt * width;
+        }
+        return true;
+    }
+    __device__ __forceinline__ int first(const ProductArgs& g) const { return (int)((long long)g.blocks * split / g.splits); }
+    __device__ __forceinline__ int last(const ProductArgs& g) const { return (int)((long long)g.blocks * (split + 1) / g.splits); }
 };
 
 // The tensor core's two operands are the table (128 rows of b to the 128 lanes) and the queries (TM rows of a to as many
@@ -335,31 +363,86 @@ constexpr int kTileN = 128;
 constexpr int kTmemColumns = 512;
 template <int TM>
 struct Tile {
-    // Four warps reach a tile's 128 lanes; from 64 columns on eight share them, two to a scheduler.
-    static constexpr int kColumnWarps = TM >= 64 ? 2 : 1;
+    // Four warps reach a tile's 128 lanes, and take 64 of its columns.
+    static constexpr int kColumnWarps = TM >= 64 ? TM / 64 : 1;
     static constexpr int kEpilogueWarps = 4 * kColumnWarps;
     static constexpr int kThreads = 32 * (2 + kEpilogueWarps);
     static constexpr int kWarpColumns = TM / kColumnWarps;
     static constexpr int kAGroups = (TM + 127) / 128;
     static constexpr int kBBytes = kTileN * kBlock, kABytes = TM * kBlock;
-    static constexpr int kStageBytes = kBBytes + kABytes + kGroupBytes * (1 + kAGroups);
-    static constexpr int kTileBytes = (kStageBytes + 1023) / 1024 * 1024;  // the swizzle wants 1024-byte boundaries
-    static constexpr int kStages = 200 * 1024 / kTileBytes < 10 ? 200 * 1024 / kTileBytes : 10;
+    // A stage of the ring: a block of the table's rows, with its exponents, and one of the queries' unless the block keeps those.
+    static constexpr int kLoneBytes = kBBytes + 1024, kPairBytes = (kBBytes + kABytes + kGroupBytes * (1 + kAGroups) + 1023) / 1024 * 1024;
+    static constexpr int kSpace = 220 * 1024, kMostStages = 10;
+    // Results on their way out, a box for each two warps: where a block keeps its queries, whose sums are short.
+    static constexpr int kBoxBytes = 4096, kBoxes = kColumnWarps * 2 * kBoxBytes;
+    static constexpr int kPairStages = kSpace / kPairBytes < kMostStages ? kSpace / kPairBytes : kMostStages;
+    static constexpr int kMostResident = 100 * 1024 / kABytes;  // blocks of the queries' rows that a block keeps
     // Two accumulators, so that a tile is written out while the next one is summed.  Two of 256 columns leave no room for scales:
     // they share 64, and the next tile begins once those are read, which are read first.
     static constexpr bool kShare = TM > 128;
     static constexpr int kNextColumns = kShare ? TM - 64 : TM < 32 ? 32 : TM;
-    static constexpr int kScaleColumns = 4 * (1 + kAGroups);
     static constexpr int kScale0 = kNextColumns + (TM < 32 ? 32 : TM);
-    static_assert(kScale0 + kStages * kScaleColumns <= kTmemColumns, "accumulators and scales share the tensor memory");
-    static constexpr size_t smem() { return 1024 + (size_t)kStages * kTileBytes; }
+    static_assert(kScale0 + kPairStages * 4 * (1 + kAGroups) <= kTmemColumns, "accumulators and scales share the tensor memory");
+    static_assert(kScale0 + (kMostResident + 3) / 4 * 4 * kAGroups + 4 * kMostStages <= kTmemColumns, "accumulators and scales share the tensor memory");
+    static int resident_bytes(int blocks) { return blocks * kABytes + (blocks + 3) / 4 * kAGroups * kGroupBytes; }
+    static int lone_stages(int blocks) { return std::min(kMostStages, (kSpace - kBoxes - (resident_bytes(blocks) + 1023) / 1024 * 1024) / kLoneBytes); }
+    static constexpr size_t smem() { return 1024 + (size_t)kSpace; }
 };
+// Where `out` takes boxes of whole lines: 64 columns of 16-bit results by 32 rows from two warps, 32 columns of fp32 by 16 rows from
+// one.  (4096 x 62 504 bf16 results of 128-wide rows: 180 us, where rows do not lie on 16 bytes and are stored 64 bytes at a time 239.)
+template <class TOut>
+constexpr int kBoxColumns = 128 / (int)sizeof(TOut);
+template <class TOut>
+constexpr int kBoxRows = sizeof(TOut) == 4 ? 16 : 32;
 
 __device__ __forceinline__ void bulk_load(uint8_t* dst_smem, const void* src, uint32_t bytes, uint64_t* bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                  ::"r"(tc::smem_u32(dst_smem)), "l"(src), "r"(bytes), "r"(tc::smem_u32(bar))
                  : "memory");
 }
+__device__ __forceinline__ void box_store(const CUtensorMap* map, const uint8_t* src_smem, int x, int y) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];"
+                 ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(tc::smem_u32(src_smem))
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ void box_stores_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }  // they have left shared memory
+__device__ __forceinline__ void box_stores_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+__device__ __forceinline__ void two_warps_sync(int which) { asm volatile("bar.sync %0, 64;" ::"r"(1 + which) : "memory"); }
+// Whether any of two warps' threads says so: they meet at barriers of their own from here on, so they go on or end together.
+__device__ __forceinline__ bool two_warps_any(int which, bool mine) {
+    uint32_t any;
+    asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 p, %2, 0;\nbar.red.or.pred q, %1, 64, p;\nselp.u32 %0, 1, 0, q;\n}" : "=r"(any) : "r"(1 + which), "r"((uint32_t)mine) : "memory");
+    return any != 0;
+}
+// 16 lanes by 32 columns of TMEM, a fragment of 8 x 8 for each two registers: thread t has lane t / 4 (registers 0, 1 of four) or
+// t / 4 + 8 (2, 3) and columns 2 (t % 4) and the next, of eight columns for each four registers.  Does not wait.
+__device__ __forceinline__ void tmem_ld_fragments(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+          "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// Four fragments of 16-bit values, each turned: lane i gives the address of row i % 8 of fragment i / 8.
+__device__ __forceinline__ void store_turned(uint32_t smem, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(smem), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+template <class T>
+__device__ __forceinline__ uint32_t rounded_pair(uint32_t lo, uint32_t hi);
+template <>
+__device__ __forceinline__ uint32_t rounded_pair<__half>(uint32_t lo, uint32_t hi) {
+    const __half2 v = __floats2half2_rn(__uint_as_float(lo), __uint_as_float(hi));
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <>
+__device__ __forceinline__ uint32_t rounded_pair<__nv_bfloat16>(uint32_t lo, uint32_t hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(__uint_as_float(lo), __uint_as_float(hi));
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
 // 32 rows of 16 bytes in shared memory (rows 16 bytes apart, groups of 8 rows 128) to 4 columns of TMEM, once for each of the
 // four groups of 32 lanes: where block_scale reads the scales of 128 rows and 4 blocks.
 __device__ __forceinline__ void copy_scales(uint32_t tmem, uint32_t smem) {
@@ -418,21 +501,24 @@ __device__ __forceinline__ void store_columns(TOut* out, long long stride, const
 }
 
 // Warp 0 fetches, warp 1 multiplies, the others write out; a block takes one tile after another, and its next tile is fetched
-// and multiplied while the last one is written.
-template <int TM, class TOut>
+// and multiplied while the last one is written.  RESIDENT: the block's rows of `a` fit its shared memory beside the ring and are
+// fetched once (512 x 500 000 x 256: per tile 32 KB of the table from L2 instead of 96).
+template <int TM, class TOut, bool RESIDENT>
 static __global__ void __launch_bounds__(Tile<TM>::kThreads, 1)
-k_product8(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap b_map, ProductArgs g) {
+k_product8(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap b_map, const __grid_constant__ CUtensorMap out_map, ProductArgs g) {
     using L = Tile<TM>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    __shared__ uint64_t s_full[L::kStages], s_empty[L::kStages], s_done[2], s_free[2];  // s_free[0] alone where accumulators share columns
+    __shared__ uint64_t s_full[L::kMostStages], s_empty[L::kMostStages], s_done[2], s_free[2];  // s_free[0] alone where accumulators share columns
+    __shared__ uint64_t s_resident;
     __shared__ uint32_t s_tmem;
     __shared__ int s_gave_up;
     volatile int* const gave_up = &s_gave_up;
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < L::kStages; ++i) tc::mbar_init(&s_full[i], 1), tc::mbar_init(&s_empty[i], 1);
+        for (int i = 0; i < g.stages; ++i) tc::mbar_init(&s_full[i], 1), tc::mbar_init(&s_empty[i], 1);
         for (int i = 0; i < 2; ++i) tc::mbar_init(&s_done[i], 1), tc::mbar_init(&s_free[i], L::kEpilogueWarps);
+        tc::mbar_init(&s_resident, 1);
         tc::mbar_fence_init();
         s_gave_up = 0;
     }
@@ -442,31 +528,44 @@ k_product8(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CU
     tc::tc_fence_after();
     grid_dependency_sync();
     const uint32_t tmem = s_tmem;
-    const int n_work = g.n_tiles * g.m_tiles * g.splits;
+    // resident: [blocks][TM][128] values, exponents, then the ring
+    constexpr int kTileBytes = RESIDENT ? L::kLoneBytes : L::kPairBytes;
+    const int a_exponents = g.blocks * L::kABytes;
+    uint8_t* const ring = RESIDENT ? smem + (a_exponents + g.groups * L::kAGroups * kGroupBytes + 1023) / 1024 * 1024 : smem;
+    uint8_t* const boxes = smem + L::kSpace - L::kBoxes;
+    // of the rows past the last group of 128 any group's scales will do: their values are zeros that no one stores
+    const auto a_group = [&](int mt, int i, int group) {
+        return g.a_exponents + ((size_t)min(mt * L::kAGroups + i, (g.m - 1) / 128) * g.groups + group) * kGroupBytes;
+    };
 
     if (warp == 0) {
         if (tc::elect_one()) {
             int stage = 0;
             uint32_t parity = 1;  // the ring starts empty
-            for (int w = blockIdx.x; w < n_work; w += gridDim.x) {
-                const TilePlace tile(g, w);
-                const int mt = tile.mt, nt = tile.nt, split = tile.split;
-                const int first = (int)((long long)g.blocks * split / g.splits), last = (int)((long long)g.blocks * (split + 1) / g.splits);
+            Tiles<RESIDENT> tile(g);
+            if (RESIDENT && tile.n_work > 0) {
+                tc::mbar_arrive_expect(&s_resident, (uint32_t)(a_exponents + g.groups * L::kAGroups * kGroupBytes));
+                for (int kb = 0; kb < g.blocks; ++kb) tc::tma_load_2d(smem + kb * L::kABytes, &a_map, kb * kBlock, tile.mt * TM, &s_resident);
+                for (int group = 0; group < g.groups; ++group)
+                    for (int i = 0; i < L::kAGroups; ++i)
+                        bulk_load(smem + a_exponents + (group * L::kAGroups + i) * kGroupBytes, a_group(tile.mt, i, group), kGroupBytes, &s_resident);
+            }
+            for (; tile.here(g); tile.w += tile.step) {
+                const int first = tile.first(g), last = tile.last(g);
                 for (int kb = first; kb < last; ++kb) {
                     if (!wait(&s_empty[stage], parity, gave_up)) goto fetched;
-                    uint8_t* const at = smem + stage * L::kTileBytes;
-                    tc::mbar_arrive_expect(&s_full[stage], L::kStageBytes);
-                    tc::tma_load_2d(at, &b_map, kb * kBlock, nt * kTileN, &s_full[stage]);
-                    tc::tma_load_2d(at + L::kBBytes, &a_map, kb * kBlock, mt * TM, &s_full[stage]);
-                    uint8_t* const scales = at + L::kBBytes + L::kABytes;
-                    bulk_load(scales, g.b_exponents + ((size_t)nt * g.groups + kb / 4) * kGroupBytes, kGroupBytes, &s_full[stage]);
+                    uint8_t* const at = ring + stage * kTileBytes;
+                    tc::mbar_arrive_expect(&s_full[stage], L::kBBytes + kGroupBytes + (RESIDENT ? 0 : L::kABytes + L::kAGroups * kGroupBytes));
+                    tc::tma_load_2d(at, &b_map, kb * kBlock, tile.nt * kTileN, &s_full[stage]);
+                    bulk_load(at + L::kBBytes, g.b_exponents + ((size_t)tile.nt * g.groups + kb / 4) * kGroupBytes, kGroupBytes, &s_full[stage]);
+                    if (!RESIDENT) {
+                        uint8_t* const a = at + L::kBBytes + 1024;
+                        tc::tma_load_2d(a, &a_map, kb * kBlock, tile.mt * TM, &s_full[stage]);
 #pragma unroll
-                    for (int i = 0; i < L::kAGroups; ++i) {
-                        // rows past the last group of 128: any group's scales will do, their values are zeros that no one stores
-                        const int row_group = min(mt * L::kAGroups + i, (g.m - 1) / 128);
-                        bulk_load(scales + kGroupBytes * (1 + i), g.a_exponents + ((size_t)row_group * g.groups + kb / 4) * kGroupBytes, kGroupBytes, &s_full[stage]);
+                        for (int i = 0; i < L::kAGroups; ++i)
+                            bulk_load(i == 0 ? at + L::kBBytes + kGroupBytes : a + L::kABytes, a_group(tile.mt, i, kb / 4), kGroupBytes, &s_full[stage]);
                     }
-                    if (++stage == L::kStages) stage = 0, parity ^= 1;
+                    if (++stage == g.stages) stage = 0, parity ^= 1;
                 }
             }
         fetched:;
@@ -475,25 +574,36 @@ k_product8(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CU
         if (tc::elect_one()) {
             int stage = 0, slot = 0;
             uint32_t parity = 0, slot_parity = 1;
-            for (int w = blockIdx.x; w < n_work; w += gridDim.x) {
-                const int split = w / (g.m_tiles * g.n_tiles);
-                const int first = (int)((long long)g.blocks * split / g.splits), last = (int)((long long)g.blocks * (split + 1) / g.splits);
+            const uint32_t a_scales = tmem + L::kScale0, ring_scales = a_scales + (RESIDENT ? g.groups * 4 * L::kAGroups : 0);
+            Tiles<RESIDENT> tile(g);
+            if (RESIDENT && tile.n_work > 0) {
+                if (!wait(&s_resident, 0, gave_up)) goto multiplied;
+                tc::tc_fence_after();
+                for (int i = 0; i < g.groups * L::kAGroups; ++i) copy_scales(a_scales + 4 * i, tc::smem_u32(smem + a_exponents + i * kGroupBytes));
+            }
+            for (; tile.here(g); tile.w += tile.step) {
+                const int first = tile.first(g), last = tile.last(g);
                 if (!wait(&s_free[L::kShare ? 0 : slot], slot_parity, gave_up)) goto multiplied;
                 tc::tc_fence_after();
                 for (int kb = first; kb < last; ++kb) {
                     if (!wait(&s_full[stage], parity, gave_up)) goto multiplied;
                     tc::tc_fence_after();
-                    const uint32_t at = tc::smem_u32(smem + stage * L::kTileBytes);
-                    const uint32_t scales = tmem + L::kScale0 + stage * L::kScaleColumns;
+                    const uint32_t at = tc::smem_u32(ring + stage * kTileBytes);
+                    const uint32_t b_scale = ring_scales + stage * 4 * (RESIDENT ? 1 : 1 + L::kAGroups);
+                    const uint32_t a_scale = RESIDENT ? a_scales + (kb / 4) * 4 * L::kAGroups : b_scale + 4;
+                    copy_scales(b_scale, at + L::kBBytes);
+                    if (!RESIDENT) {
 #pragma unroll
-                    for (int i = 0; i < 1 + L::kAGroups; ++i) copy_scales(scales + 4 * i, at + L::kBBytes + L::kABytes + kGroupBytes * i);
-                    const uint64_t b_desc = tc::make_kmajor_sw128_desc(at), a_desc = tc::make_kmajor_sw128_desc(at + L::kBBytes);
+                        for (int i = 0; i < L::kAGroups; ++i) copy_scales(a_scale + 4 * i, i == 0 ? at + L::kBBytes + kGroupBytes : at + L::kBBytes + 1024 + L::kABytes);
+                    }
+                    const uint64_t b_desc = tc::make_kmajor_sw128_desc(at);
+                    const uint64_t a_desc = tc::make_kmajor_sw128_desc(RESIDENT ? tc::smem_u32(smem + kb * L::kABytes) : at + L::kBBytes + 1024);
                     const uint32_t idesc = scaled_idesc(kTileN, TM, kb & 3);
 #pragma unroll
                     for (int q = 0; q < 4; ++q)  // 32 values of k each, 32 bytes further
-                        mma_scaled(tmem + slot * L::kNextColumns, b_desc + 2 * q, a_desc + 2 * q, idesc, scales, scales + 4, kb > first || q > 0);
+                        mma_scaled(tmem + slot * L::kNextColumns, b_desc + 2 * q, a_desc + 2 * q, idesc, b_scale, a_scale, kb > first || q > 0);
                     tc::umma_commit(&s_empty[stage]);
-                    if (++stage == L::kStages) stage = 0, parity ^= 1;
+                    if (++stage == g.stages) stage = 0, parity ^= 1;
                 }
                 tc::umma_commit(&s_done[slot]);
                 slot ^= 1;
@@ -503,37 +613,83 @@ k_product8(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CU
         }
     } else {
         const int quad = warp & 3;  // the lanes that this warp may read
-        const int column0 = (warp - 2) / 4 * L::kWarpColumns;
+        const int part = (warp - 2) / 4, column0 = part * L::kWarpColumns, pair = 2 * part + quad / 2;
+        constexpr int kRows = L::kWarpColumns < 32 ? L::kWarpColumns : 32, kChunks = L::kWarpColumns / kRows;
+        constexpr bool kStage = TM >= 64 && RESIDENT, kWide = sizeof(TOut) == 4;  // fp32 boxes are one warp's
+        uint8_t* const box = boxes + pair * L::kBoxBytes + (kWide ? quad % 2 * (L::kBoxBytes / 2) : 0);
+        const bool issues = lane == 0 && (kWide || quad % 2 == 0);
         int slot = 0;
         uint32_t parity = 0;
-        for (int w = blockIdx.x; w < n_work; w += gridDim.x) {
-            const TilePlace tile(g, w);
-            const int mt = tile.mt, nt = tile.nt, split = tile.split;
-            if (!wait(&s_done[slot], parity, gave_up)) break;
+        for (Tiles<RESIDENT> tile(g); tile.here(g); tile.w += tile.step) {
+            if (two_warps_any(pair, !wait(&s_done[slot], parity, gave_up))) break;
             tc::tc_fence_after();
-            const int n = nt * kTileN + quad * 32 + lane, m0 = mt * TM + column0;
-            TOut* const out = static_cast<TOut*>(g.out) + (size_t)split * g.split_stride + (long long)m0 * g.out_stride + n;
-            // of shared columns the warps that read them read them first: the last 64 of slot 0, the first 64 of slot 1
-            const int first = L::kShare && slot == 0 && column0 > 0 ? 64 : 0;
+            const int n0 = tile.nt * kTileN + quad * 32, m0 = tile.mt * TM + column0;
+            // of shared columns those that read them, the last 64 of slot 0 and the first 64 of slot 1, hold up the next tile
+            const bool holds = !L::kShare || part == (slot == 0 ? L::kColumnWarps - 1 : 0);
             const auto release = [&] {
                 tc::tc_fence_before();
                 __syncwarp();
                 if (lane == 0) tc::mbar_arrive(&s_free[L::kShare ? 0 : slot]);
             };
-            if (L::kShare && (slot == 0) == (column0 == 0)) release();  // this warp reads none of them
-#pragma unroll 1
-            for (int i = 0; i < L::kWarpColumns; i += 32) {
-                const int c = i ^ first;
-                uint32_t acc[32];
-                tc::tmem_ld32(tmem + slot * L::kNextColumns + column0 + c + ((uint32_t)(quad * 32) << 16), acc);
-                if (L::kShare ? i == 32 && (slot == 0) != (column0 == 0) : i + 32 >= L::kWarpColumns) release();
-                constexpr int kRows = L::kWarpColumns < 32 ? L::kWarpColumns : 32;
-                const int rows = min(kRows, g.m - m0 - c);
-                store_columns<kRows>(out + (long long)c * g.out_stride, g.out_stride, acc, n < g.n ? rows : 0);
+            if (!holds) release();
+            const uint32_t taddr = tmem + slot * L::kNextColumns + column0 + ((uint32_t)(quad * 32) << 16);
+            bool stored = false;
+            if constexpr (kStage && !kWide) {
+                if (g.staged) {
+                    uint32_t lo[kChunks][16], hi[kChunks][16];
+#pragma unroll
+                    for (int i = 0; i < kChunks; ++i) tmem_ld_fragments(taddr + 32 * i, lo[i]), tmem_ld_fragments(taddr + 32 * i + (16u << 16), hi[i]);
+                    tmem_ld_wait();
+                    if (holds) release();
+                    stored = true;
+#pragma unroll
+                    for (int i = 0; i < kChunks; ++i) {
+                        if (m0 + 32 * i >= g.m) break;  // the same for both warps
+                        if (issues) box_stores_read();
+                        two_warps_sync(pair);
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {  // eight rows of `out` each, of 16 bytes for each eight lanes
+                            const uint32_t at = tc::smem_u32(box) + (q * 8 + (lane & 7)) * 128 + (((quad % 2 * 4 + lane / 8) ^ (lane & 7)) << 4);
+                            store_turned(at, rounded_pair<TOut>(lo[i][4 * q], lo[i][4 * q + 1]), rounded_pair<TOut>(lo[i][4 * q + 2], lo[i][4 * q + 3]),
+                                         rounded_pair<TOut>(hi[i][4 * q], hi[i][4 * q + 1]), rounded_pair<TOut>(hi[i][4 * q + 2], hi[i][4 * q + 3]));
+                        }
+                        tc::fence_async_shared();
+                        two_warps_sync(pair);
+                        if (issues && n0 < g.n) box_store(&out_map, box, n0, m0 + 32 * i);
+                    }
+                }
+            }
+            if (!stored) {
+                uint32_t acc[kChunks][32];
+#pragma unroll
+                for (int i = 0; i < kChunks; ++i) tc::tmem_ld32(taddr + 32 * i, acc[i]);
+                if (holds) release();
+                TOut* const out = static_cast<TOut*>(g.out) + (size_t)tile.split * g.split_stride + (long long)m0 * g.out_stride + n0 + lane;
+#pragma unroll
+                for (int i = 0; i < kChunks; ++i) {
+                    const int rows = min(kRows, g.m - m0 - 32 * i);
+                    if (kStage && kWide && g.staged) {
+#pragma unroll
+                        for (int h = 0; h < 32; h += kBoxRows<TOut>) {
+                            if (h >= rows) break;
+                            if (issues) box_stores_read();
+                            __syncwarp();
+                            TOut* const to = reinterpret_cast<TOut*>(box) + lane;
+#pragma unroll
+                            for (int q = 0; q < kBoxRows<TOut>; ++q) lp::store_rounded(to + q * 32, __uint_as_float(acc[i][(h + q) % 32]));
+                            tc::fence_async_shared();
+                            __syncwarp();
+                            if (issues && n0 < g.n) box_store(&out_map, box, n0, m0 + 32 * i + h);
+                        }
+                    } else {
+                        store_columns<kRows>(out + (long long)(32 * i) * g.out_stride, g.out_stride, acc[i], n0 + lane < g.n ? rows : 0);
+                    }
+                }
             }
             slot ^= 1;
             if (slot == 0) parity ^= 1;
         }
+        if (kStage && g.staged && issues) box_stores_done();
     }
     tc::tc_fence_before();
     __syncthreads();
