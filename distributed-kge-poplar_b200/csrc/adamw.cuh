@@ -53,9 +53,6 @@ __device__ __forceinline__ float max_or_nan(float a, float b) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
     return y;
 }
-// To bf16, toward zero or away from it, as an fp32.  An infinity stays one; a NaN's bits would run over.
-__device__ __forceinline__ float rounded_stochastically(float x, uint32_t r16) { return __uint_as_float((__float_as_uint(x) + r16) & 0xffff0000u); }
-
 // The codes of a block: TOP = 255 without a sign, 127 with one.  They are kept short: at 60 integer instructions a value a step in 8
 // bits was bound by them at three times the time that its bytes take.
 template <int TOP>
@@ -68,20 +65,26 @@ template <int TOP>
 __device__ __forceinline__ uint32_t code_base(int exponent) { return (uint32_t)(8 * exponent + 7 - TOP) << 20; }
 template <int TOP>
 __device__ __forceinline__ float decode(uint32_t byte, uint32_t base) {
-    uint32_t bits = (byte << 20) + base;
-    if (TOP == 127) bits += (byte >> 7) * 0x78000000u;  // the sign from bit 27 to bit 31
-    return (byte & (uint32_t)TOP) ? __uint_as_float(bits) : 0.f;
+    const uint32_t code = TOP == 127 ? byte & 127u : byte;
+    const uint32_t bits = code * 0x100000u + min(code, 1u) * base;  // multiplications have a pipe of their own
+    return __uint_as_float(TOP == 127 ? (byte * 0x1000000u & 0x80000000u) | bits : bits);
 }
-// The code of a value of a finite block; none is above TOP, since the block's exponent is that of its largest value rounded up.
+// The code of a value of a finite block in the upper byte; none is above TOP, since the block's exponent is that of its largest value
+// rounded up.  A sign is not added yet.
 template <int TOP>
 __device__ __forceinline__ uint32_t encode(float x, uint32_t base, uint32_t r16) {
-    const uint32_t b = __float_as_uint(x), magnitude = TOP == 127 ? b & 0x7fffffffu : b;
-    const int least = TOP == 255 ? (int)(min(magnitude, 1u) << 20) : 0;
-    const uint32_t code = (uint32_t)max((int)(r16 * 16u + (magnitude - base)), least) >> 20;
-    return TOP == 127 ? code | (b >> 24 & 128u) : code;
+    const uint32_t magnitude = TOP == 127 ? __float_as_uint(x) & 0x7fffffffu : __float_as_uint(x);
+    const int least = TOP == 255 ? (int)(min(magnitude, 1u) * 0x100000u) : 0;
+    return (uint32_t)max((int)(r16 * 16u + (magnitude - base)), least) * 16u;
 }
-__device__ __forceinline__ uint32_t four_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+__device__ __forceinline__ uint32_t upper_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __byte_perm(__byte_perm(a, b, 0x0073), __byte_perm(c, d, 0x0073), 0x5410);
+}
+template <int TOP>
+__device__ __forceinline__ uint32_t encode_four(const float* x, uint32_t base, const uint32_t* r16) {
+    const uint32_t codes = upper_bytes(encode<TOP>(x[0], base, r16[0]), encode<TOP>(x[1], base, r16[1]), encode<TOP>(x[2], base, r16[2]), encode<TOP>(x[3], base, r16[3]));
+    if (TOP == 255) return codes;
+    return codes | (upper_bytes(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])) & 0x80808080u);
 }
 
 __device__ __forceinline__ float value(const float* p) { return *p; }
@@ -187,17 +190,37 @@ struct Step {
 };
 // Bits 8 to 23 of a draw.
 __device__ __forceinline__ uint32_t middle(uint32_t draw) { return __byte_perm(draw, 0, 0x4421); }
-template <int N>
-__device__ __forceinline__ void round_all(float (&p)[N], const uint32_t (&draw)[N]) {
-    float sum = 0.f;
+// Four values rounded as their draws say, as they are stored.  fp32 ones are not rounded.
+template <class TP>
+__device__ __forceinline__ Quad<TP> rounded_quad(const float (&p)[4], const uint32_t (&draw)[4]) {
+    Quad<TP> out;
+    if constexpr (sizeof(TP) == 4) {
+        out.set(p);
+    } else {
+        uint32_t b[4];
 #pragma unroll
-    for (int j = 0; j < N; ++j) sum += fabsf(p[j]);
-    const bool finite = sum < INFINITY;  // else one by one: a NaN's bits would run over
+        for (int j = 0; j < 4; ++j) b[j] = __float_as_uint(p[j]) + middle(draw[j]);
+        if (!(fabsf(p[0]) + fabsf(p[1]) + (fabsf(p[2]) + fabsf(p[3])) < INFINITY)) {  // an infinity stays one; a NaN's bits would run over
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-        const float rounded = rounded_stochastically(p[j], middle(draw[j]));
-        p[j] = finite || p[j] == p[j] ? rounded : __uint_as_float(0x7fc00000u);
+            for (int j = 0; j < 4; ++j) b[j] = p[j] == p[j] ? b[j] : 0x7fc00000u;
+        }
+        out.raw.x = __byte_perm(b[0], b[1], 0x7632);
+        out.raw.y = __byte_perm(b[2], b[3], 0x7632);
     }
+    return out;
+}
+// The lane's values go back, `live` of them.
+template <class T>
+__device__ __forceinline__ void store_quad(T* p, const Quad<T>& q, int live, bool whole) {
+    if (whole) {
+        *reinterpret_cast<decltype(q.raw)*>(p) = q.raw;
+        return;
+    }
+    float v[4];
+    q.floats(v);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (j < live) put(p + j, v[j]);
 }
 
 // Moments in fp32: a warp takes 128 values at a time, four to a lane, and two such units, fetched together.
@@ -242,31 +265,70 @@ static __global__ void __launch_bounds__(kThreads, 3) k_adamw32(const __grid_con
         // past the tensor's end gradient and moments are 0, and stay so
 #pragma unroll
         for (int j = 0; j < 4; ++j) step.take(p[j], g[j], m[j], v[j]);
+        uint32_t draw[4] = {};
         if constexpr (sizeof(TP) == 2) {
-            uint32_t draw[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) draw[j] = mix(step.mixed(at[u]) + (uint32_t)j * 0x9E3779B9u);
-            round_all(p, draw);
         }
-        if (whole[u]) {
-            Quad<TP> out;
-            out.set(p);
-            *reinterpret_cast<decltype(out.raw)*>(param[u]) = out.raw;
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (j < live[u]) put(param[u] + j, p[j]);
-        }
+        store_quad(param[u], rounded_quad<TP>(p, draw), live[u], whole[u]);
         *reinterpret_cast<float4*>(adam_m + at[u]) = make_float4(m[0], m[1], m[2], m[3]);
         *reinterpret_cast<float4*>(adam_v + at[u]) = make_float4(v[0], v[1], v[2], v[3]);
     }
 }
 
+// A lane's 16 values, fetched and stored 16 bytes at a time (of 16-bit types 8 at a time left every sector to four accesses: 192 us for
+// 60 million bf16 parameters, WIDE us so).
+template <class T>
+struct LaneValues {
+    static constexpr int kVectors = 16 * (int)sizeof(T) / 16;
+    uint4 raw[kVectors];
+    __device__ __forceinline__ void load(const T* p, int live, bool whole) {
+        if (whole) {
+#pragma unroll
+            for (int i = 0; i < kVectors; ++i) raw[i] = reinterpret_cast<const uint4*>(p)[i];
+        } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                Quad<T> part;
+                load_quad(part, p + 4 * q, live - 4 * q, false);
+                set(q, part);
+            }
+        }
+    }
+    __device__ __forceinline__ void store(T* p, int live, bool whole) const {
+        if (whole) {
+#pragma unroll
+            for (int i = 0; i < kVectors; ++i) reinterpret_cast<uint4*>(p)[i] = raw[i];
+        } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) store_quad(p + 4 * q, quad(q), live - 4 * q, false);
+        }
+    }
+    __device__ __forceinline__ Quad<T> quad(int q) const {
+        Quad<T> part;
+        if constexpr (sizeof(T) == 4) {
+            part.raw = make_float4(__uint_as_float(raw[q].x), __uint_as_float(raw[q].y), __uint_as_float(raw[q].z), __uint_as_float(raw[q].w));
+        } else {
+            part.raw = q & 1 ? make_uint2(raw[q / 2].z, raw[q / 2].w) : make_uint2(raw[q / 2].x, raw[q / 2].y);
+        }
+        return part;
+    }
+    __device__ __forceinline__ void set(int q, const Quad<T>& part) {
+        if constexpr (sizeof(T) == 4) {
+            raw[q] = make_uint4(__float_as_uint(part.raw.x), __float_as_uint(part.raw.y), __float_as_uint(part.raw.z), __float_as_uint(part.raw.w));
+        } else if (q & 1) {
+            raw[q / 2].z = part.raw.x, raw[q / 2].w = part.raw.y;
+        } else {
+            raw[q / 2].x = part.raw.x, raw[q / 2].y = part.raw.y;
+        }
+    }
+};
+
 // Moments in 8 bits: a warp takes four blocks of 128 values, eight lanes and 16 values a lane each, so that what a lane does but once
 // (finding its place, the exponents) is spread over 16 values: with four a lane a step took 92 instructions a value.
 constexpr int kLaneValues = 16;
 template <class TP, class TG, int MAX>
-static __global__ void __launch_bounds__(kThreads, 2) k_adamw8(const __grid_constant__ Table<MAX> table, Params a, uint8_t* __restrict__ adam_m, uint8_t* __restrict__ adam_v,
+static __global__ void __launch_bounds__(kThreads, 3) k_adamw8(const __grid_constant__ Table<MAX> table, Params a, uint8_t* __restrict__ adam_m, uint8_t* __restrict__ adam_v,
                                                                uint8_t* __restrict__ m_exponent, uint8_t* __restrict__ v_exponent) {
     constexpr int N = kLaneValues;
     grid_dependency_sync();
@@ -281,8 +343,8 @@ static __global__ void __launch_bounds__(kThreads, 2) k_adamw8(const __grid_cons
     const bool whole = live == N && t.aligned;
     TP* const param = static_cast<TP*>(t.param) + i0;
     const TG* const grad = static_cast<const TG*>(t.grad) + i0;
-    Quad<TP> p_raw[N / 4];
-    Quad<TG> g_raw[N / 4];
+    LaneValues<TP> params;
+    LaneValues<TG> grads;
     uint4 m_raw = make_uint4(0, 0, 0, 0), v_raw = m_raw;
     int em = 16, ev = 33;
     if (here) {
@@ -290,8 +352,8 @@ static __global__ void __launch_bounds__(kThreads, 2) k_adamw8(const __grid_cons
         v_raw = *reinterpret_cast<const uint4*>(adam_v + at);
         em = m_exponent[block], ev = v_exponent[block];
     }
-#pragma unroll
-    for (int q = 0; q < N / 4; ++q) load_quad(p_raw[q], static_cast<const TP*>(param) + 4 * q, live - 4 * q, whole), load_quad(g_raw[q], grad + 4 * q, live - 4 * q, whole);
+    params.load(param, live, whole);
+    grads.load(grad, live, whole);
     const Step step(a);
     float m[N], v[N], largest_m = 0.f, largest_v = 0.f;
     uint32_t draw[N];
@@ -314,8 +376,8 @@ static __global__ void __launch_bounds__(kThreads, 2) k_adamw8(const __grid_cons
     for (int q = 0; q < N / 4; ++q) {
         float p[4], g[4];
         uint32_t d[4];
-        p_raw[q].floats(p);
-        g_raw[q].floats(g);
+        params.quad(q).floats(p);
+        grads.quad(q).floats(g);
         // past the tensor's end gradient and moments are 0, and stay so
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -324,17 +386,9 @@ static __global__ void __launch_bounds__(kThreads, 2) k_adamw8(const __grid_cons
             largest_m = max_or_nan(largest_m, fabsf(m[4 * q + j]));
             largest_v = max_or_nan(largest_v, v[4 * q + j]);
         }
-        if constexpr (sizeof(TP) == 2) round_all(p, d);
-        if (whole) {
-            Quad<TP> out;
-            out.set(p);
-            *reinterpret_cast<decltype(out.raw)*>(param + 4 * q) = out.raw;
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (4 * q + j < live) put(param + 4 * q + j, p[j]);
-        }
+        params.set(q, rounded_quad<TP>(p, d));
     }
+    params.store(param, live, whole);
     uint32_t top_m = __float_as_uint(largest_m), top_v = __float_as_uint(largest_v);
 #pragma unroll
     for (int o = 4; o > 0; o >>= 1) top_m = max(top_m, __shfl_xor_sync(~0u, top_m, o)), top_v = max(top_v, __shfl_xor_sync(~0u, top_v, o));
@@ -344,13 +398,10 @@ static __global__ void __launch_bounds__(kThreads, 2) k_adamw8(const __grid_cons
     uint32_t mw[4], vw[4];
 #pragma unroll
     for (int q = 0; q < N / 4; ++q) {
-        uint32_t c[4], d[4];
+        uint32_t low[4], high[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            c[j] = encode<127>(m[4 * q + j], base_m, draw[4 * q + j] & 0xffffu);
-            d[j] = encode<255>(v[4 * q + j], base_v, draw[4 * q + j] >> 16);
-        }
-        mw[q] = four_bytes(c[0], c[1], c[2], c[3]), vw[q] = four_bytes(d[0], d[1], d[2], d[3]);
+        for (int j = 0; j < 4; ++j) low[j] = draw[4 * q + j] & 0xffffu, high[j] = draw[4 * q + j] >> 16;
+        mw[q] = encode_four<127>(m + 4 * q, base_m, low), vw[q] = encode_four<255>(v + 4 * q, base_v, high);
     }
     *reinterpret_cast<uint4*>(adam_m + at) = make_uint4(mw[0], mw[1], mw[2], mw[3]);
     *reinterpret_cast<uint4*>(adam_v + at) = make_uint4(vw[0], vw[1], vw[2], vw[3]);
@@ -359,25 +410,27 @@ static __global__ void __launch_bounds__(kThreads, 2) k_adamw8(const __grid_cons
 
 static __global__ void __launch_bounds__(kThreads) k_moments(const uint8_t* __restrict__ adam_m, const uint8_t* __restrict__ m_exponent,
                                                              const uint8_t* __restrict__ adam_v, const uint8_t* __restrict__ v_exponent,
-                                                             size_t blocks, __nv_bfloat16* __restrict__ m_out, __nv_bfloat16* __restrict__ v_out) {
-    const size_t block = (size_t)blockIdx.x * (kThreads / 32) + threadIdx.x / 32;
-    if (block >= blocks) return;
-    const size_t at = block * kBlock + (threadIdx.x & 31) * 4;
-    const uint32_t cm = *reinterpret_cast<const uint32_t*>(adam_m + at), cv = *reinterpret_cast<const uint32_t*>(adam_v + at);
-    const int em = m_exponent[block], ev = v_exponent[block];
-    const uint32_t base_m = code_base<127>(em), base_v = code_base<255>(ev);
-    const float nan = __uint_as_float(0x7fc00000u);
-    float m[4], v[4];
+                                                             size_t size, __nv_bfloat16* __restrict__ m_out, __nv_bfloat16* __restrict__ v_out) {
+    grid_dependency_sync();
+    const size_t at = ((size_t)blockIdx.x * kThreads + threadIdx.x) * 8;  // eight values a thread: 16 bytes of results
+    if (at >= size) return;
+    const uint2 mw = *reinterpret_cast<const uint2*>(adam_m + at), vw = *reinterpret_cast<const uint2*>(adam_v + at);
+    const int em = m_exponent[at / kBlock], ev = v_exponent[at / kBlock];
+    const uint32_t base_m = code_base<127>(em), base_v = code_base<255>(ev), words[4] = {mw.x, mw.y, vw.x, vw.y};
+    uint32_t bits[4][4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        m[j] = em == 255 ? nan : decode<127>(cm >> (8 * j) & 255u, base_m);
-        v[j] = ev == 255 ? nan : decode<255>(cv >> (8 * j) & 255u, base_v);
-    }
-    Quad<__nv_bfloat16> out;
-    out.set(m);
-    *reinterpret_cast<uint2*>(m_out + at) = out.raw;
-    out.set(v);
-    *reinterpret_cast<uint2*>(v_out + at) = out.raw;
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t byte = __byte_perm(words[i], 0, 0x4440 + j);
+            bits[i][j] = (i < 2 ? em : ev) == 255 ? 0x7fc00000u : __float_as_uint(i < 2 ? decode<127>(byte, base_m) : decode<255>(byte, base_v));
+        }
+    const auto packed = [&](int i) {
+        return make_uint4(__byte_perm(bits[i][0], bits[i][1], 0x7632), __byte_perm(bits[i][2], bits[i][3], 0x7632), __byte_perm(bits[i + 1][0], bits[i + 1][1], 0x7632),
+                          __byte_perm(bits[i + 1][2], bits[i + 1][3], 0x7632));
+    };
+    *reinterpret_cast<uint4*>(m_out + at) = packed(0);
+    *reinterpret_cast<uint4*>(v_out + at) = packed(2);
 }
 
 }  // namespace adamw

@@ -413,10 +413,10 @@ void adamw_moments(const uint8_t* adam_m, const uint8_t* m_exponent, const uint8
     if (size == 0) return;
     need(adam_m && m_exponent && adam_v && v_exponent && m_bf16 && v_bf16, "kge_op_adamw_moments: null argument");
     need(aligned_to(adam_m, 16) && aligned_to(adam_v, 16) && aligned_to(m_bf16, 16) && aligned_to(v_bf16, 16), "kge_op_adamw_moments: moments must be aligned to 16 bytes");
-    const size_t blocks = size / adamw::kBlock, per = adamw::kThreads / 32;
-    adamw::k_moments<<<grid_of((blocks + per - 1) / per, what), adamw::kThreads, 0, stream>>>(adam_m, m_exponent, adam_v, v_exponent, blocks,
-                                                                                            static_cast<__nv_bfloat16*>(m_bf16), static_cast<__nv_bfloat16*>(v_bf16));
-    KGE_CUDA(cudaGetLastError());
+    const size_t per = adamw::kThreads * 8;
+    const cudaError_t err = launch_dependent(adamw::k_moments, dim3(grid_of((size + per - 1) / per, what)), dim3(adamw::kThreads), 0, stream, adam_m, m_exponent, adam_v,
+                                             v_exponent, size, static_cast<__nv_bfloat16*>(m_bf16), static_cast<__nv_bfloat16*>(v_bf16));
+    KGE_CUDA(err);
 }
 
 }  // namespace kge
