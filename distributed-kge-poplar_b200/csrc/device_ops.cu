@@ -238,27 +238,28 @@ constexpr CUtensorMapDataType map_type() {
     return sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
 }
 
+template <int TM, class TOut, bool RESIDENT>
+void launch_product(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& out, const rows8::ProductArgs& g, int grid, cudaStream_t stream) {
+    using L = rows8::Tile<TM, RESIDENT>;
+    allow_shared_memory<rows8::k_product8<TM, TOut, RESIDENT>>(L::smem());
+    const cudaError_t err = launch_dependent(rows8::k_product8<TM, TOut, RESIDENT>, dim3(grid), dim3(L::kThreads), L::smem(), stream, a, b, out, g);
+    KGE_CUDA(err);
+}
 template <int TM, class TOut>
 void launch_product(const CUtensorMap& a, const CUtensorMap& b, rows8::ProductArgs g, cudaStream_t stream) {
-    using L = rows8::Tile<TM>;
-    CUtensorMap out = b;  // where results are stored directly, any map
-    const bool resident = g.blocks <= L::kMostResident && g.splits == 1 && g.m_tiles <= kSmCount;
-    g.stages = resident ? L::lone_stages(g.blocks) : L::kPairStages;
-    g.staged = TM >= 64 && resident && aligned_to(g.out, 16) && (g.m == 1 || g.out_stride * (long long)sizeof(TOut) % 16 == 0);
-    if (g.staged)
-        out = encoded_map(map_type<TOut>(), g.out, (cuuint64_t)g.n, (cuuint64_t)g.m, round_up((size_t)std::max<long long>(g.out_stride, g.n) * sizeof(TOut), 16),
-                          rows8::kBoxColumns<TOut>, rows8::kBoxRows<TOut>, sizeof(TOut) == 4 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B);
-    cudaError_t err;
-    if (resident) {
-        allow_shared_memory<rows8::k_product8<TM, TOut, true>>(L::smem());
-        const int grid = std::min(g.n_tiles, kSmCount / g.m_tiles) * g.m_tiles;
-        err = launch_dependent(rows8::k_product8<TM, TOut, true>, dim3(grid), dim3(L::kThreads), L::smem(), stream, a, b, out, g);
+    using Kept = rows8::Tile<TM, true>;
+    if (g.blocks <= Kept::kMostResident && g.splits == 1 && g.m_tiles <= kSmCount) {
+        CUtensorMap out = b;  // where results are stored directly, any map
+        g.stages = Kept::lone_stages(g.blocks);
+        g.staged = TM >= 64 && aligned_to(g.out, 16) && (g.m == 1 || g.out_stride * (long long)sizeof(TOut) % 16 == 0);
+        if (g.staged)
+            out = encoded_map(map_type<TOut>(), g.out, (cuuint64_t)g.n, (cuuint64_t)g.m, round_up((size_t)std::max<long long>(g.out_stride, g.n) * sizeof(TOut), 16),
+                              rows8::kBoxColumns<TOut>, rows8::kBoxRows<TOut>, sizeof(TOut) == 4 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B);
+        launch_product<TM, TOut, true>(a, b, out, g, std::min(g.n_tiles, kSmCount / g.m_tiles) * g.m_tiles, stream);
     } else {
-        allow_shared_memory<rows8::k_product8<TM, TOut, false>>(L::smem());
-        const int work = g.n_tiles * g.m_tiles * g.splits;
-        err = launch_dependent(rows8::k_product8<TM, TOut, false>, dim3(std::min(work, kSmCount)), dim3(L::kThreads), L::smem(), stream, a, b, out, g);
+        g.stages = rows8::Tile<TM, false>::kPairStages;
+        launch_product<TM, TOut, false>(a, b, b, g, std::min(g.n_tiles * g.m_tiles * g.splits, kSmCount), stream);
     }
-    KGE_CUDA(err);
 }
 template <class TOut>
 void launch_product(int tile_m, const CUtensorMap& a, const CUtensorMap& b, const rows8::ProductArgs& g, cudaStream_t stream) {

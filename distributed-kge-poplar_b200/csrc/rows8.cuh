@@ -361,10 +361,14 @@ struct Tiles {
 // of them at once.
 constexpr int kTileN = 128;
 constexpr int kTmemColumns = 512;
-template <int TM>
+// Blocks of k that are summed in tensor memory before the sum joins the others in registers: there every addition rounds toward
+// zero, which takes 1e-5 off a sum of 16 384 positive products and 5e-7 off one of 2048.
+constexpr int kSegment = 16;
+template <int TM, bool RESIDENT>
 struct Tile {
-    // Four warps reach a tile's 128 lanes, and take 64 of its columns.
-    static constexpr int kColumnWarps = TM >= 64 ? TM / 64 : 1;
+    // Four warps reach a tile's 128 lanes, and take 64 of its columns; 128 where long sums are kept in registers: sixteen warps have 96
+    // registers each, eight 168.
+    static constexpr int kColumnWarps = TM < 64 ? 1 : TM == 256 && !RESIDENT ? 2 : TM / 64;
     static constexpr int kEpilogueWarps = 4 * kColumnWarps;
     static constexpr int kThreads = 32 * (2 + kEpilogueWarps);
     static constexpr int kWarpColumns = TM / kColumnWarps;
@@ -377,6 +381,7 @@ struct Tile {
     static constexpr int kBoxBytes = 4096, kBoxes = kColumnWarps * 2 * kBoxBytes;
     static constexpr int kPairStages = kSpace / kPairBytes < kMostStages ? kSpace / kPairBytes : kMostStages;
     static constexpr int kMostResident = 100 * 1024 / kABytes;  // blocks of the queries' rows that a block keeps
+    static constexpr bool kOneSegment = RESIDENT && kMostResident <= kSegment;
     // Two accumulators, so that a tile is written out while the next one is summed.  Two of 256 columns leave no room for scales:
     // they share 64, and the next tile begins once those are read, which are read first.
     static constexpr bool kShare = TM > 128;
@@ -425,21 +430,28 @@ __device__ __forceinline__ void tmem_ld_fragments(uint32_t taddr, uint32_t (&r)[
         : "r"(taddr)
         : "memory");
 }
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr)
+                 : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 // Four fragments of 16-bit values, each turned: lane i gives the address of row i % 8 of fragment i / 8.
 __device__ __forceinline__ void store_turned(uint32_t smem, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(smem), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 template <class T>
-__device__ __forceinline__ uint32_t rounded_pair(uint32_t lo, uint32_t hi);
+__device__ __forceinline__ uint32_t rounded_pair(float lo, float hi);
 template <>
-__device__ __forceinline__ uint32_t rounded_pair<__half>(uint32_t lo, uint32_t hi) {
-    const __half2 v = __floats2half2_rn(__uint_as_float(lo), __uint_as_float(hi));
+__device__ __forceinline__ uint32_t rounded_pair<__half>(float lo, float hi) {
+    const __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 template <>
-__device__ __forceinline__ uint32_t rounded_pair<__nv_bfloat16>(uint32_t lo, uint32_t hi) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(__uint_as_float(lo), __uint_as_float(hi));
+__device__ __forceinline__ uint32_t rounded_pair<__nv_bfloat16>(float lo, float hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 
@@ -480,23 +492,23 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile in
 
 // One column of the tile per row of `out`.  With a row's address and a test for each store a tile took 5.8 us, a dependent chain
 // of some ten instructions a store with one warp to a scheduler; four addresses apart and no tests leave two.
-template <int ROWS, class TOut>
-__device__ __forceinline__ void store_columns(TOut* out, long long stride, const uint32_t (&acc)[32], int rows) {
+template <int ROWS, class TOut, int N>
+__device__ __forceinline__ void store_columns(TOut* out, long long stride, const float (&acc)[N], int rows) {
     if (rows == ROWS) {
         TOut *p0 = out, *p1 = out + stride, *p2 = p1 + stride, *p3 = p2 + stride;
         const long long four = 4 * stride;
 #pragma unroll
         for (int j = 0; j < ROWS; j += 4) {
-            lp::store_rounded(p0, __uint_as_float(acc[j]));
-            lp::store_rounded(p1, __uint_as_float(acc[j + 1]));
-            lp::store_rounded(p2, __uint_as_float(acc[j + 2]));
-            lp::store_rounded(p3, __uint_as_float(acc[j + 3]));
+            lp::store_rounded(p0, acc[j]);
+            lp::store_rounded(p1, acc[j + 1]);
+            lp::store_rounded(p2, acc[j + 2]);
+            lp::store_rounded(p3, acc[j + 3]);
             p0 += four, p1 += four, p2 += four, p3 += four;
         }
     } else {
 #pragma unroll
         for (int j = 0; j < ROWS; ++j)
-            if (j < rows) lp::store_rounded(out + j * stride, __uint_as_float(acc[j]));
+            if (j < rows) lp::store_rounded(out + j * stride, acc[j]);
     }
 }
 
@@ -504,9 +516,9 @@ __device__ __forceinline__ void store_columns(TOut* out, long long stride, const
 // and multiplied while the last one is written.  RESIDENT: the block's rows of `a` fit its shared memory beside the ring and are
 // fetched once (512 x 500 000 x 256: per tile 32 KB of the table from L2 instead of 96).
 template <int TM, class TOut, bool RESIDENT>
-static __global__ void __launch_bounds__(Tile<TM>::kThreads, 1)
+static __global__ void __launch_bounds__(Tile<TM, RESIDENT>::kThreads, 1)
 k_product8(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap b_map, const __grid_constant__ CUtensorMap out_map, ProductArgs g) {
-    using L = Tile<TM>;
+    using L = Tile<TM, RESIDENT>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     __shared__ uint64_t s_full[L::kMostStages], s_empty[L::kMostStages], s_done[2], s_free[2];  // s_free[0] alone where accumulators share columns
@@ -582,114 +594,179 @@ k_product8(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CU
                 for (int i = 0; i < g.groups * L::kAGroups; ++i) copy_scales(a_scales + 4 * i, tc::smem_u32(smem + a_exponents + i * kGroupBytes));
             }
             for (; tile.here(g); tile.w += tile.step) {
-                const int first = tile.first(g), last = tile.last(g);
-                if (!wait(&s_free[L::kShare ? 0 : slot], slot_parity, gave_up)) goto multiplied;
-                tc::tc_fence_after();
-                for (int kb = first; kb < last; ++kb) {
-                    if (!wait(&s_full[stage], parity, gave_up)) goto multiplied;
+                const int last = tile.last(g);
+                for (int kb = tile.first(g); kb < last;) {
+                    if (!wait(&s_free[L::kShare ? 0 : slot], slot_parity, gave_up)) goto multiplied;
                     tc::tc_fence_after();
-                    const uint32_t at = tc::smem_u32(ring + stage * kTileBytes);
-                    const uint32_t b_scale = ring_scales + stage * 4 * (RESIDENT ? 1 : 1 + L::kAGroups);
-                    const uint32_t a_scale = RESIDENT ? a_scales + (kb / 4) * 4 * L::kAGroups : b_scale + 4;
-                    copy_scales(b_scale, at + L::kBBytes);
-                    if (!RESIDENT) {
+                    const int segment = kb, end = min(last, kb + kSegment);
+                    for (; kb < end; ++kb) {
+                        if (!wait(&s_full[stage], parity, gave_up)) goto multiplied;
+                        tc::tc_fence_after();
+                        const uint32_t at = tc::smem_u32(ring + stage * kTileBytes);
+                        const uint32_t b_scale = ring_scales + stage * 4 * (RESIDENT ? 1 : 1 + L::kAGroups);
+                        const uint32_t a_scale = RESIDENT ? a_scales + (kb / 4) * 4 * L::kAGroups : b_scale + 4;
+                        copy_scales(b_scale, at + L::kBBytes);
+                        if (!RESIDENT) {
 #pragma unroll
-                        for (int i = 0; i < L::kAGroups; ++i) copy_scales(a_scale + 4 * i, i == 0 ? at + L::kBBytes + kGroupBytes : at + L::kBBytes + 1024 + L::kABytes);
+                            for (int i = 0; i < L::kAGroups; ++i)
+                                copy_scales(a_scale + 4 * i, i == 0 ? at + L::kBBytes + kGroupBytes : at + L::kBBytes + 1024 + L::kABytes);
+                        }
+                        const uint64_t b_desc = tc::make_kmajor_sw128_desc(at);
+                        const uint64_t a_desc = tc::make_kmajor_sw128_desc(RESIDENT ? tc::smem_u32(smem + kb * L::kABytes) : at + L::kBBytes + 1024);
+                        const uint32_t idesc = scaled_idesc(kTileN, TM, kb & 3);
+#pragma unroll
+                        for (int q = 0; q < 4; ++q)  // 32 values of k each, 32 bytes further
+                            mma_scaled(tmem + slot * L::kNextColumns, b_desc + 2 * q, a_desc + 2 * q, idesc, b_scale, a_scale, kb > segment || q > 0);
+                        tc::umma_commit(&s_empty[stage]);
+                        if (++stage == g.stages) stage = 0, parity ^= 1;
                     }
-                    const uint64_t b_desc = tc::make_kmajor_sw128_desc(at);
-                    const uint64_t a_desc = tc::make_kmajor_sw128_desc(RESIDENT ? tc::smem_u32(smem + kb * L::kABytes) : at + L::kBBytes + 1024);
-                    const uint32_t idesc = scaled_idesc(kTileN, TM, kb & 3);
-#pragma unroll
-                    for (int q = 0; q < 4; ++q)  // 32 values of k each, 32 bytes further
-                        mma_scaled(tmem + slot * L::kNextColumns, b_desc + 2 * q, a_desc + 2 * q, idesc, b_scale, a_scale, kb > first || q > 0);
-                    tc::umma_commit(&s_empty[stage]);
-                    if (++stage == g.stages) stage = 0, parity ^= 1;
+                    tc::umma_commit(&s_done[slot]);
+                    slot ^= 1;
+                    if (L::kShare || slot == 0) slot_parity ^= 1;
                 }
-                tc::umma_commit(&s_done[slot]);
-                slot ^= 1;
-                if (L::kShare || slot == 0) slot_parity ^= 1;
             }
         multiplied:;
         }
     } else {
         const int quad = warp & 3;  // the lanes that this warp may read
         const int part = (warp - 2) / 4, column0 = part * L::kWarpColumns, pair = 2 * part + quad / 2;
-        constexpr int kRows = L::kWarpColumns < 32 ? L::kWarpColumns : 32, kChunks = L::kWarpColumns / kRows;
-        constexpr bool kStage = TM >= 64 && RESIDENT, kWide = sizeof(TOut) == 4;  // fp32 boxes are one warp's
-        uint8_t* const box = boxes + pair * L::kBoxBytes + (kWide ? quad % 2 * (L::kBoxBytes / 2) : 0);
-        const bool issues = lane == 0 && (kWide || quad % 2 == 0);
         int slot = 0;
         uint32_t parity = 0;
-        for (Tiles<RESIDENT> tile(g); tile.here(g); tile.w += tile.step) {
-            if (two_warps_any(pair, !wait(&s_done[slot], parity, gave_up))) break;
-            tc::tc_fence_after();
-            const int n0 = tile.nt * kTileN + quad * 32, m0 = tile.mt * TM + column0;
-            // of shared columns those that read them, the last 64 of slot 0 and the first 64 of slot 1, hold up the next tile
-            const bool holds = !L::kShare || part == (slot == 0 ? L::kColumnWarps - 1 : 0);
-            const auto release = [&] {
-                tc::tc_fence_before();
-                __syncwarp();
-                if (lane == 0) tc::mbar_arrive(&s_free[L::kShare ? 0 : slot]);
-            };
-            if (!holds) release();
-            const uint32_t taddr = tmem + slot * L::kNextColumns + column0 + ((uint32_t)(quad * 32) << 16);
-            bool stored = false;
-            if constexpr (kStage && !kWide) {
-                if (g.staged) {
-                    uint32_t lo[kChunks][16], hi[kChunks][16];
-#pragma unroll
-                    for (int i = 0; i < kChunks; ++i) tmem_ld_fragments(taddr + 32 * i, lo[i]), tmem_ld_fragments(taddr + 32 * i + (16u << 16), hi[i]);
-                    tmem_ld_wait();
-                    if (holds) release();
-                    stored = true;
-#pragma unroll
-                    for (int i = 0; i < kChunks; ++i) {
-                        if (m0 + 32 * i >= g.m) break;  // the same for both warps
-                        if (issues) box_stores_read();
-                        two_warps_sync(pair);
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) {  // eight rows of `out` each, of 16 bytes for each eight lanes
-                            const uint32_t at = tc::smem_u32(box) + (q * 8 + (lane & 7)) * 128 + (((quad % 2 * 4 + lane / 8) ^ (lane & 7)) << 4);
-                            store_turned(at, rounded_pair<TOut>(lo[i][4 * q], lo[i][4 * q + 1]), rounded_pair<TOut>(lo[i][4 * q + 2], lo[i][4 * q + 3]),
-                                         rounded_pair<TOut>(hi[i][4 * q], hi[i][4 * q + 1]), rounded_pair<TOut>(hi[i][4 * q + 2], hi[i][4 * q + 3]));
-                        }
-                        tc::fence_async_shared();
-                        two_warps_sync(pair);
-                        if (issues && n0 < g.n) box_store(&out_map, box, n0, m0 + 32 * i);
+        if constexpr (RESIDENT) {
+            constexpr int kRows = L::kWarpColumns < 32 ? L::kWarpColumns : 32, kChunks = L::kWarpColumns / kRows;
+            constexpr bool kStage = TM >= 64, kWide = sizeof(TOut) == 4;  // fp32 boxes are one warp's
+            uint8_t* const box = boxes + pair * L::kBoxBytes + (kWide ? quad % 2 * (L::kBoxBytes / 2) : 0);
+            const bool issues = lane == 0 && (kWide || quad % 2 == 0);
+            const bool fragments = kStage && !kWide && g.staged;
+            for (Tiles<RESIDENT> tile(g); tile.here(g); tile.w += tile.step) {
+                const int n0 = tile.nt * kTileN + quad * 32, m0 = tile.mt * TM + column0;
+                float acc[kChunks][32];  // 32 columns each, a lane's or (to be turned) two fragments of 16 lanes
+                bool ended = false;
+                for (int kb = 0; kb < g.blocks; kb += kSegment) {
+                    if (two_warps_any(pair, !wait(&s_done[slot], parity, gave_up))) {
+                        ended = true;
+                        break;
                     }
-                }
-            }
-            if (!stored) {
-                uint32_t acc[kChunks][32];
+                    tc::tc_fence_after();
+                    // of shared columns those that read them, the last 64 of slot 0 and the first 64 of slot 1, hold up the next tile
+                    const bool holds = !L::kShare || part == (slot == 0 ? L::kColumnWarps - 1 : 0);
+                    const auto release = [&] {
+                        tc::tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) tc::mbar_arrive(&s_free[L::kShare ? 0 : slot]);
+                    };
+                    if (!holds) release();
+                    const uint32_t taddr = tmem + slot * L::kNextColumns + column0 + ((uint32_t)(quad * 32) << 16);
+                    uint32_t sum[kChunks][32];
+                    if (fragments) {
+                        uint32_t lo[kChunks][16], hi[kChunks][16];
 #pragma unroll
-                for (int i = 0; i < kChunks; ++i) tc::tmem_ld32(taddr + 32 * i, acc[i]);
-                if (holds) release();
-                TOut* const out = static_cast<TOut*>(g.out) + (size_t)tile.split * g.split_stride + (long long)m0 * g.out_stride + n0 + lane;
+                        for (int i = 0; i < kChunks; ++i) tmem_ld_fragments(taddr + 32 * i, lo[i]), tmem_ld_fragments(taddr + 32 * i + (16u << 16), hi[i]);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < kChunks; ++i)
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) sum[i][j] = lo[i][j], sum[i][16 + j] = hi[i][j];
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < kChunks; ++i) tc::tmem_ld32(taddr + 32 * i, sum[i]);
+                    }
+                    if (holds) release();
+#pragma unroll
+                    for (int i = 0; i < kChunks; ++i)
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) acc[i][j] = L::kOneSegment || kb == 0 ? __uint_as_float(sum[i][j]) : acc[i][j] + __uint_as_float(sum[i][j]);
+                    slot ^= 1;
+                    if (slot == 0) parity ^= 1;
+                }
+                if (ended) break;
+                TOut* const out = static_cast<TOut*>(g.out) + (long long)m0 * g.out_stride + n0 + lane;
 #pragma unroll
                 for (int i = 0; i < kChunks; ++i) {
                     const int rows = min(kRows, g.m - m0 - 32 * i);
-                    if (kStage && kWide && g.staged) {
-#pragma unroll
-                        for (int h = 0; h < 32; h += kBoxRows<TOut>) {
-                            if (h >= rows) break;
+                    if (rows <= 0) break;  // the same for both warps
+                    if (kStage && g.staged) {
+                        if constexpr (kStage && !kWide) {
                             if (issues) box_stores_read();
-                            __syncwarp();
-                            TOut* const to = reinterpret_cast<TOut*>(box) + lane;
+                            two_warps_sync(pair);
 #pragma unroll
-                            for (int q = 0; q < kBoxRows<TOut>; ++q) lp::store_rounded(to + q * 32, __uint_as_float(acc[i][(h + q) % 32]));
+                            for (int q = 0; q < 4; ++q) {  // eight rows of `out` each, of 16 bytes for each eight lanes
+                                const uint32_t at = tc::smem_u32(box) + (q * 8 + (lane & 7)) * 128 + (((quad % 2 * 4 + lane / 8) ^ (lane & 7)) << 4);
+                                const float* const lo = acc[i] + 4 * q;
+                                const float* const hi = acc[i] + 16 + 4 * q;
+                                store_turned(at, rounded_pair<TOut>(lo[0], lo[1]), rounded_pair<TOut>(lo[2], lo[3]), rounded_pair<TOut>(hi[0], hi[1]), rounded_pair<TOut>(hi[2], hi[3]));
+                            }
                             tc::fence_async_shared();
-                            __syncwarp();
-                            if (issues && n0 < g.n) box_store(&out_map, box, n0, m0 + 32 * i + h);
+                            two_warps_sync(pair);
+                            if (issues && n0 < g.n) box_store(&out_map, box, n0, m0 + 32 * i);
+                        } else if constexpr (kStage) {
+#pragma unroll
+                            for (int h = 0; h < 32; h += kBoxRows<TOut>) {
+                                if (h >= rows) break;
+                                if (issues) box_stores_read();
+                                __syncwarp();
+                                TOut* const to = reinterpret_cast<TOut*>(box) + lane;
+#pragma unroll
+                                for (int q = 0; q < kBoxRows<TOut>; ++q) lp::store_rounded(to + q * 32, acc[i][(h + q) % 32]);
+                                tc::fence_async_shared();
+                                __syncwarp();
+                                if (issues && n0 < g.n) box_store(&out_map, box, n0, m0 + 32 * i + h);
+                            }
                         }
                     } else {
                         store_columns<kRows>(out + (long long)(32 * i) * g.out_stride, g.out_stride, acc[i], n0 + lane < g.n ? rows : 0);
                     }
                 }
             }
-            slot ^= 1;
-            if (slot == 0) parity ^= 1;
+            if (kStage && g.staged && issues) box_stores_done();
+        } else {
+            // the columns in halves; the upper warps begin with their second one, which is where columns are shared
+            constexpr int kHalf = L::kWarpColumns / 2;
+            const int turned = L::kShare && part == 1 ? 1 : 0;
+            for (Tiles<RESIDENT> tile(g); tile.here(g); tile.w += tile.step) {
+                float acc[2][kHalf];
+#pragma unroll
+                for (int i = 0; i < kHalf; ++i) acc[0][i] = acc[1][i] = 0.f;
+                const int last = tile.last(g);
+                bool ended = false;
+                for (int kb = tile.first(g); kb < last; kb += kSegment) {
+                    if (__any_sync(~0u, !wait(&s_done[slot], parity, gave_up))) {
+                        ended = true;
+                        break;
+                    }
+                    tc::tc_fence_after();
+                    const bool holds = !L::kShare || part != slot;
+                    const auto release = [&] {
+                        tc::tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) tc::mbar_arrive(&s_free[L::kShare ? 0 : slot]);
+                    };
+                    if (!holds) release();
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t taddr = tmem + slot * L::kNextColumns + column0 + (h ^ turned) * kHalf + ((uint32_t)(quad * 32) << 16);
+#pragma unroll
+                        for (int i = 0; i < kHalf; i += 8) {
+                            uint32_t sum[8];
+                            tmem_ld8(taddr + i, sum);
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) acc[h][i + j] += __uint_as_float(sum[j]);
+                        }
+                        if (holds && h == (L::kShare ? 0 : 1)) release();
+                    }
+                    slot ^= 1;
+                    if (slot == 0) parity ^= 1;
+                }
+                if (ended) break;
+                const int n = tile.nt * kTileN + quad * 32 + lane;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int m0 = tile.mt * TM + column0 + (h ^ turned) * kHalf;
+                    TOut* const out = static_cast<TOut*>(g.out) + (size_t)tile.split * g.split_stride + (long long)m0 * g.out_stride + n;
+                    store_columns<kHalf>(out, g.out_stride, acc[h], n < g.n ? min(kHalf, g.m - m0) : 0);
+                }
+            }
         }
-        if (kStage && g.staged && issues) box_stores_done();
     }
     tc::tc_fence_before();
     __syncthreads();

@@ -363,6 +363,18 @@ def test_product8_of_long_sums_and_few_tiles(ops):
         assert torch.equal(ops.product8(a, b), got)
 
 
+@pytest.mark.parametrize("m,n,k", [(130, 300, 70_000), (600, 2000, 17_000), (20, 140, 9000)])
+def test_product8_of_sums_that_only_grow(ops, m, n, k):
+    """2048 products are summed in tensor memory, whose additions round toward zero: with all of one sign that takes at most their
+    number of instructions, 64, times half of 2^-23 on average off the sum; those sums are joined in fp32, rounded to nearest.  One sum
+    over all of k was 6e-5 off at 65 536."""
+    g = gen(k)
+    a, b = (ops.quantise_rows(torch.rand(rows, k, generator=g).cuda()) for rows in (m, n))
+    got = ops.product8(a, b).double()
+    want = a.dequantise().double() @ b.dequantise().double().T
+    assert float(((got - want) / want).abs().max()) <= 64 * 2.0**-24 + math.sqrt(k / 2048) * 2.0**-22
+
+
 def test_product8_with_values_that_are_not_finite(ops):
     x, y = torch.randn(20, 200), torch.randn(150, 200)
     x[3, 5], y[140, 199] = math.inf, math.nan
