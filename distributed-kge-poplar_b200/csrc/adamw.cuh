@@ -276,8 +276,7 @@ static __global__ void __launch_bounds__(kThreads, 3) k_adamw32(const __grid_con
     }
 }
 
-// A lane's 16 values, fetched and stored 16 bytes at a time (of 16-bit types 8 at a time left every sector to four accesses: 192 us for
-// 60 million bf16 parameters, WIDE us so).
+// A lane's 16 values, fetched and stored 16 bytes at a time.
 template <class T>
 struct LaneValues {
     static constexpr int kVectors = 16 * (int)sizeof(T) / 16;

@@ -63,9 +63,10 @@ lp::Scores checked_scores(const kge_scores& s, const char* what) {
 
 namespace {
 
-// A row is one block's, of as many threads as give each SM 1024 (lp_rank: 128 rows of 100 003 bf16 scores with lists of 100 take
-// LPRANK1 us by blocks of 1024 threads and LPRANK4 in parts of 256), unless there are so few rows that they are cut into parts, four to an
-// SM, or a row's groups of vectors do not fit a block's shared memory.
+// A row is one block's, of as many threads as give each SM 1024: 128 rows of 100 003 bf16 scores with lists of 100 take 16 us by blocks
+// of 1024 threads, and in parts of 256 with a second kernel to join them 29.  Rows are cut into parts, four to an SM, where there are too
+// few of them for that (4 rows of 2 500 001 fp32 scores: 26 us, by one block each 713) or their groups of vectors do not fit a block's
+// shared memory.
 struct LogProbsPlan {
     int threads, parts, vectors;
     size_t sums_bytes, bytes;

@@ -335,12 +335,13 @@ int kge_op_log_probs_grad(const kge_scores* scores, const float* row_state, cons
  * of zeros), and is held as value * 2^-e rounded to 4 exponent and 3 significand bits (e4m3, to nearest, ties to even).  A
  * power of two costs such a format nothing but half an octave of its range, and the tensor core applies it as it multiplies.
  * NaN and infinities are held as NaN.
- *   values     [rows, ld] bytes, ld = cols rounded up to 16 (bytes past cols are 0); aligned to 16 bytes
+ *   values     [rows, ld] bytes, ld = cols rounded up to 16, of more than 128 columns to 128 (bytes past cols are 0); aligned to
+ *              16 bytes
  *   exponents  e + 127 in the order in which the tensor core takes them: 512 bytes for each group of 128 rows and 4 blocks, in
  *              them byte (r % 32) * 16 + (r / 32) * 4 + block % 4 of the group's row r; groups of a row side by side; aligned
  *              to 16 bytes.  Bytes of rows and blocks that do not exist are 127.
  * kge_op_rows8_bytes gives the sizes of both.  x [rows, cols] has any row stride of at least cols elements; with `transposed`
- * the rows that are made are the columns of x: values [cols, ld] with ld = rows rounded up to 16, blocks along a column.
+ * the rows that are made are the columns of x: values [cols, ld] with ld that of `rows` columns, blocks along a column.
  */
 int kge_op_rows8_bytes(size_t rows, size_t cols, size_t* values, size_t* exponents);
 int kge_op_quantise_rows(const void* x, int float_type, size_t rows, size_t cols, long long row_stride, int transposed,

@@ -66,7 +66,8 @@ def test_outputs_that_are_refused():
 def test_rows8_that_are_refused():
     values, exponents = C.c_size_t(), C.c_size_t()
     assert lib.kge_op_rows8_bytes(129, 513, C.byref(values), C.byref(exponents)) == capi.OK
-    assert (values.value, exponents.value) == (129 * 528, 2 * 2 * 512)
+    assert (values.value, exponents.value) == (129 * 640, 2 * 2 * 512)
+    assert lib.kge_op_rows8_bytes(3, 17, C.byref(values), C.byref(exponents)) == capi.OK and values.value == 3 * 32
     refused(lib.kge_op_rows8_bytes(1, 1, None, C.byref(exponents)), "null argument")
     quantise = lib.kge_op_quantise_rows
     refused(quantise(SOME, capi.U32, 4, 10, 10, 0, SOME, SOME, None), "element type")
