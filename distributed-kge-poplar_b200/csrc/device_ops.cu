@@ -49,7 +49,7 @@ lp::Scores checked_scores(const kge_scores& s, const char* what) {
     const size_t bytes = type_bytes(s.float_type, what);
     if (s.cols > kMostColumns) fail(KGE_INVALID_ARGUMENT, msg() << what << ": " << s.cols << " columns, " << kMostColumns << " are the most");
     if (s.rows > 1 && s.row_stride < (long long)s.cols) fail(KGE_INVALID_ARGUMENT, msg() << what << ": rows of " << s.cols << " columns, " << s.row_stride << " apart");
-    if (!(s.scale > 0.f) || !std::isfinite(s.scale)) fail(KGE_INVALID_ARGUMENT, msg() << what << ": scale must be positive and finite, not " << s.scale);
+    if (!(s.scale > 0.f) || !std::isfinite(s.scale * lp::kLog2e)) fail(KGE_INVALID_ARGUMENT, msg() << what << ": scale must be positive and finite, not " << s.scale);
     if (s.rows && s.cols && !s.x) fail(KGE_INVALID_ARGUMENT, msg() << what << ": null scores");
     if (!aligned_to(s.x, bytes)) fail(KGE_INVALID_ARGUMENT, msg() << what << ": scores are not aligned to their type");
     if (s.mask && s.mask_stride != 0 && s.rows > 1 && s.mask_stride < (long long)s.cols)

@@ -68,7 +68,8 @@ def check_log_probs(got, want, cols, entropy_scale=1.0):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("rows,cols,n_best", [(1, 1, 1), (3, 1, 4), (2, 7, 10), (5, 63, 5), (1, 1387, 10), (4, 2049, 128), (7, 4097, 100), (2, 40_003, 17), (3, 100_001, 128)])
+@pytest.mark.parametrize("rows,cols,n_best", [(1, 1, 1), (3, 1, 4), (2, 7, 10), (5, 63, 5), (1, 1387, 10), (4, 2049, 128), (7, 4097, 100), (2, 40_003, 17), (3, 100_001, 128),
+                                              (40, 20_001, 30), (20, 90_003, 100), (200, 9000, 100), (400, 5000, 128)])
 def test_log_probs(ops, rows, cols, n_best, dtype):
     g = gen(rows * 1000 + cols)
     x = (torch.randn(rows, cols, generator=g) * 3).to(dtype)
@@ -117,6 +118,18 @@ def test_log_probs_of_rows_in_parts(ops, rows, cols, n_best, dtype):
         check_log_probs(got, forms.log_probs(x, target, count=c, n_best=n_best), cols)
         again = ops.log_probs(x.cuda(), target.cuda(), count=cuda(c), n_best=n_best)
         assert torch.equal(got.log_sum, again.log_sum) and torch.equal(got.entropy, again.entropy)
+
+
+@pytest.mark.parametrize("rows,cols", [(3, 200), (400, 5000), (200, 9000), (20, 60_000)])
+def test_log_probs_of_rows_of_equal_scores(ops, rows, cols):
+    """Every size of block: all columns reach any threshold, and the lowest are listed."""
+    x = torch.zeros(rows, cols)
+    x[1, cols // 2 :] = 2.0
+    got = ops.log_probs(x.cuda(), n_best=100)
+    want = torch.arange(100, dtype=torch.int32).repeat(rows, 1)
+    want[1] += cols // 2
+    assert torch.equal(got.best_index.cpu(), want)
+    check_log_probs(got, forms.log_probs(x, None, n_best=100), cols)
 
 
 def test_log_probs_of_equal_scores_in_many_parts(ops):
@@ -644,3 +657,45 @@ def test_calls_on_two_streams_at_once(ops):
     for v, r, p in got:
         w, q = want[0 if v is x[0] else 1]
         assert torch.equal(r.log_prob, w.log_prob) and torch.equal(r.entropy, w.entropy) and torch.equal(r.best_index, w.best_index) and torch.equal(p, q)
+
+
+def test_calls_that_are_refused(ops):
+    x = torch.randn(6, 8).cuda()
+    r = ops.log_probs(x, n_best=2)
+    column = torch.zeros(8, 6).cuda().T
+    for call, text in [(lambda: ops.log_probs(column), "contiguous along its rows"), (lambda: ops.log_probs(x[0]), "two dimensions"),
+                       (lambda: ops.log_probs(x.double()), "not torch.float64"), (lambda: ops.log_probs(x[:1].expand(6, 8)), "apart"),
+                       (lambda: ops.log_probs(x, torch.zeros(6).cuda()), "torch.int32"), (lambda: ops.log_probs(x, torch.zeros(5, dtype=torch.int32).cuda()), "shape"),
+                       (lambda: ops.log_probs(x, torch.zeros(6, dtype=torch.int32)), "on a GPU"), (lambda: ops.log_probs(x, torch.zeros(12, dtype=torch.int32).cuda()[::2]), "contiguous"),
+                       (lambda: ops.log_probs(x, mask=torch.ones(6, 7, dtype=torch.bool).cuda()), "shape"), (lambda: ops.log_probs(x, mask=x), "torch.bool"),
+                       (lambda: ops.log_probs(x, scale=0.0), "scale"), (lambda: ops.log_probs(x, scale=3e38), "scale"), (lambda: ops.log_probs(x, n_best=-1), "n_best"),
+                       (lambda: ops.log_probs_grad(x[:5], r), "shape"), (lambda: ops.log_probs_grad(x, r, grad_log_prob=torch.ones(6).cuda().half()), "torch.float32"),
+                       (lambda: ops.log_probs_grad(x, r, grad_best=torch.ones(6, 3).cuda()), "shape"), (lambda: ops.log_probs_grad(x, r, out=x.half()), "out must be"),
+                       (lambda: ops.log_probs_grad(x[:, :7], ops.log_probs(x[:, :7]), out=x[:, 1:]), "overlap"),
+                       (lambda: ops.quantise_rows(column), "contiguous along its rows"), (lambda: ops.product8(x, x[:, :4]), "rows of 8 and of 4"),
+                       (lambda: ops.product8(x, x, dtype=torch.float64), "dtype"), (lambda: ops.product8(x, x, out=torch.zeros(6, 5).cuda()), "shape"),
+                       (lambda: ops.AdamW([x, x[2:4]]), "overlap"), (lambda: ops.AdamW([x, x.bfloat16()]), "an optimiser for each type"), (lambda: ops.AdamW([x.half()]), "parameter 0 must be"),
+                       (lambda: ops.AdamW([column]), "contiguous"), (lambda: ops.AdamW([x], beta_v=1.0), "beta"), (lambda: ops.AdamW([x], epsilon=0.0), "epsilon")]:
+        with pytest.raises(ValueError, match=text):
+            call()
+    optimiser = ops.AdamW([x, torch.zeros(3).cuda()])
+    for grads, how, text in [([x], dict(learning_rate=0.1), "1 gradients for 2"), ([x, x], dict(learning_rate=0.1), "shape"), ([x.half(), torch.zeros(3).cuda()], dict(learning_rate=0.1), "others"),
+                             ([column, None], dict(learning_rate=0.1), "contiguous"), ([x, None], {}, "learning_rate or a schedule"),
+                             ([x, None], dict(schedule=torch.zeros(3).cuda()), "schedule has shape")]:
+        with pytest.raises(ValueError, match=text):
+            optimiser.step(grads, **how)
+    assert optimiser.step_count == 0
+    with pytest.raises(ValueError, match="does not fit"):
+        optimiser.load_state(ops.AdamW([x], state_bits=8).state())
+
+
+def test_gradients_that_are_broadcast_and_leaves_that_require_them(ops):
+    x = torch.randn(5, 300).cuda()
+    r = ops.log_probs(x, torch.zeros(5, dtype=torch.int32).cuda())
+    one = torch.tensor([0.25]).cuda()
+    assert torch.equal(ops.log_probs_grad(x, r, grad_log_prob=one.expand(5)), ops.log_probs_grad(x, r, grad_log_prob=torch.full((5,), 0.25).cuda()))
+    leaf = torch.randn(40, 3).cuda().requires_grad_()
+    optimiser = ops.AdamW([leaf])
+    before, version = leaf.detach().clone(), leaf._version
+    optimiser.step([torch.ones_like(leaf)], 0.1)
+    assert leaf._version > version and float((before - leaf.detach() - 0.1).abs().max()) < 1e-5
