@@ -65,7 +65,8 @@ namespace {
 
 // A row is one block's, of as many threads as give each SM 1024: 128 rows of 100 003 bf16 scores with lists of 100 take 16 us by blocks
 // of 1024 threads, and in parts of 256 with a second kernel to join them 29.  Rows are cut into parts, four to an SM, where there are too
-// few of them for that (4 rows of 2 500 001 fp32 scores: 26 us, by one block each 713) or their groups of vectors do not fit a block's
+// few of them for that (two to an SM with lists, which each part makes: 4 rows of 2 500 001 fp32 scores 24.6 us, with four 26.0, by one
+// block a row 713) or their groups of vectors do not fit a block's
 // shared memory.
 struct LogProbsPlan {
     int threads, parts, vectors;
@@ -86,7 +87,7 @@ LogProbsPlan log_probs_plan(size_t rows, size_t cols, size_t n_best, size_t widt
         while (p.threads > 256 && (size_t)p.threads * 2 > all) p.threads /= 2;  // two vectors a thread at least
         if (all > most(p.threads) || (rows <= kSmCount / 2 && (all > 16384 || (rows <= 16 && all >= 2048)))) {
             p.threads = 256;
-            parts = std::max((all + most(256) - 1) / most(256), std::min(4 * kSmCount / std::max<size_t>(1, rows), all / 1024));
+            parts = std::max((all + most(256) - 1) / most(256), std::min((n_best ? 2 : 4) * kSmCount / std::max<size_t>(1, rows), all / 1024));
         }
     }
     p.vectors = (int)std::max<size_t>(1, (all + parts - 1) / parts);
