@@ -65,9 +65,8 @@ namespace {
 
 // A row is one block's, of as many threads as give each SM 1024: 128 rows of 100 003 bf16 scores with lists of 100 take 16 us by blocks
 // of 1024 threads, and in parts of 256 with a second kernel to join them 29.  Rows are cut into parts, four to an SM, where there are too
-// few of them for that (two to an SM with lists, which each part makes: 4 rows of 2 500 001 fp32 scores 24.6 us, with four 26.0, by one
-// block a row 713) or their groups of vectors do not fit a block's
-// shared memory.
+// few of them for that or their groups of vectors do not fit a block's shared memory; two to an SM with lists, which each part makes (4
+// rows of 2 500 001 fp32 scores 24.6 us, with four to an SM 26.0, by one block a row 713).
 struct LogProbsPlan {
     int threads, parts, vectors;
     size_t sums_bytes, bytes;
@@ -210,7 +209,9 @@ ProductPlan product_plan(size_t m, size_t n, size_t k) {
     ProductPlan p;
     p.n_tiles = (int)((n + rows8::kTileN - 1) / rows8::kTileN);
     p.tile_m = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : m <= 128 ? 128 : 256;
-    // where the sum has to be split, smaller tiles need half the parts and so half the partial sums
+    // Blocks that keep their queries have a tile's 128 (512 x 500 000 x 256: 125 us, with 256, whose accumulators share columns, 143);
+    // where the sum has to be split, smaller tiles need half the parts and so half the partial sums.
+    if (p.tile_m == 256 && rows8::blocks_of(k) <= (size_t)rows8::Tile<128, true>::kMostResident && m <= (size_t)kSmCount * 128) p.tile_m = 128;
     if (p.tile_m == 256 && (long long)((m + 255) / 256) * p.n_tiles < kSmCount / 2) p.tile_m = 128;
     p.m_tiles = (int)((m + p.tile_m - 1) / p.tile_m);
     p.chunk = (int)std::min<size_t>(p.n_tiles, std::max<size_t>(16, ((size_t)32 << 20) / (rows8::kTileN * rows8::value_stride(std::max<size_t>(k, 1)))));
@@ -249,19 +250,21 @@ void launch_product(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMa
 }
 template <int TM, class TOut>
 void launch_product(const CUtensorMap& a, const CUtensorMap& b, rows8::ProductArgs g, cudaStream_t stream) {
-    using Kept = rows8::Tile<TM, true>;
-    if (g.blocks <= Kept::kMostResident && g.splits == 1 && g.m_tiles <= kSmCount) {
-        CUtensorMap out = b;  // where results are stored directly, any map
-        g.stages = Kept::lone_stages(g.blocks);
-        g.staged = TM >= 64 && aligned_to(g.out, 16) && (g.m == 1 || g.out_stride * (long long)sizeof(TOut) % 16 == 0);
-        if (g.staged)
-            out = encoded_map(map_type<TOut>(), g.out, (cuuint64_t)g.n, (cuuint64_t)g.m, round_up((size_t)std::max<long long>(g.out_stride, g.n) * sizeof(TOut), 16),
-                              rows8::kBoxColumns<TOut>, rows8::kBoxRows<TOut>, sizeof(TOut) == 4 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B);
-        launch_product<TM, TOut, true>(a, b, out, g, std::min(g.n_tiles, kSmCount / g.m_tiles) * g.m_tiles, stream);
-    } else {
-        g.stages = rows8::Tile<TM, false>::kPairStages;
-        launch_product<TM, TOut, false>(a, b, b, g, std::min(g.n_tiles * g.m_tiles * g.splits, kSmCount), stream);
+    if constexpr (TM <= 128) {
+        using Kept = rows8::Tile<TM, true>;
+        if (g.blocks <= Kept::kMostResident && g.splits == 1 && g.m_tiles <= kSmCount) {
+            CUtensorMap out = b;  // where results are stored directly, any map
+            g.stages = Kept::lone_stages(g.blocks);
+            g.boxes = TM >= 64 && aligned_to(g.out, 16) && (g.m == 1 || g.out_stride * (long long)sizeof(TOut) % 16 == 0);
+            if (g.boxes)
+                out = encoded_map(map_type<TOut>(), g.out, (cuuint64_t)g.n, (cuuint64_t)g.m, round_up((size_t)std::max<long long>(g.out_stride, g.n) * sizeof(TOut), 16),
+                                  rows8::kBoxColumns<TOut>, rows8::kBoxRows<TOut>, sizeof(TOut) == 4 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B);
+            launch_product<TM, TOut, true>(a, b, out, g, std::min(g.n_tiles, kSmCount / g.m_tiles) * g.m_tiles, stream);
+            return;
+        }
     }
+    g.stages = rows8::Tile<TM, false>::kPairStages;
+    launch_product<TM, TOut, false>(a, b, b, g, std::min(g.n_tiles * g.m_tiles * g.splits, kSmCount), stream);
 }
 template <class TOut>
 void launch_product(int tile_m, const CUtensorMap& a, const CUtensorMap& b, const rows8::ProductArgs& g, cudaStream_t stream) {

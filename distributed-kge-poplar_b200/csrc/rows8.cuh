@@ -314,12 +314,12 @@ struct ProductArgs {
     int n_tiles, m_tiles, splits;
     int chunk;  // tiles of n that are gone through for all of m before the next ones
     int stages; // of the ring
-    int staged; // 1: `out` takes whole boxes of a tile's rows
+    int boxes;  // 1: `out` takes whole boxes of a tile's rows
 };
 
 // The tiles of a block, one after another.  Tiles that are worked on at the same time lie side by side along the rows of `out`, so
-// that its memory is written in long pieces (4096 x 62 500 bf16 results of 128-wide rows: 239 us, with neighbours one above the other
-// 294), in chunks whose part of the table stays in L2 until all of m has met it.  A block that keeps its rows of `a` goes along them.
+// that its memory is written in long pieces (4096 x 62 500 bf16 results of 128-wide rows by 64 bytes of a row: 239 us, with neighbours
+// one above the other 294), in chunks whose part of the table stays in L2 until all of m has met it.  A block that keeps its rows of `a` goes along them.
 template <bool RESIDENT>
 struct Tiles {
     int w, step, n_work, stride, run;
@@ -367,9 +367,9 @@ constexpr int kTmemColumns = 512;
 constexpr int kSegment = 16;
 template <int TM, bool RESIDENT>
 struct Tile {
-    // Four warps reach a tile's 128 lanes, and take 64 of its columns; 128 where long sums are kept in registers: sixteen warps have 96
-    // registers each, eight 168.
-    static constexpr int kColumnWarps = TM < 64 ? 1 : TM == 256 && !RESIDENT ? 2 : TM / 64;
+    // Four warps reach a tile's 128 lanes, and take 64 of its columns; 128 of 256, for which eight warps have 168 registers each and
+    // sixteen would have 96.
+    static constexpr int kColumnWarps = TM <= 64 ? 1 : 2;
     static constexpr int kEpilogueWarps = 4 * kColumnWarps;
     static constexpr int kThreads = 32 * (2 + kEpilogueWarps);
     static constexpr int kWarpColumns = TM / kColumnWarps;
@@ -388,6 +388,7 @@ struct Tile {
     static constexpr bool kShare = TM > 128;
     static constexpr int kNextColumns = kShare ? TM - 64 : TM < 32 ? 32 : TM;
     static constexpr int kScale0 = kNextColumns + (TM < 32 ? 32 : TM);
+    static_assert(!RESIDENT || TM <= 128, "blocks that keep their queries have accumulators of their own, and one group of exponents");
     static_assert(kScale0 + kPairStages * 4 * (1 + kAGroups) <= kTmemColumns, "accumulators and scales share the tensor memory");
     static_assert(kScale0 + (kMostResident + 3) / 4 * 4 * kAGroups + 4 * kMostStages <= kTmemColumns, "accumulators and scales share the tensor memory");
     static int resident_bytes(int blocks) { return blocks * kABytes + (blocks + 3) / 4 * kAGroups * kGroupBytes; }
@@ -395,7 +396,7 @@ struct Tile {
     static constexpr size_t smem() { return 1024 + (size_t)kSpace; }
 };
 // Where `out` takes boxes of whole lines: 64 columns of 16-bit results by 32 rows from two warps, 32 columns of fp32 by 16 rows from
-// one.  (4096 x 62 504 bf16 results of 128-wide rows: 180 us, where rows do not lie on 16 bytes and are stored 64 bytes at a time 239.)
+// one.  (4096 x 62 504 bf16 results of 128-wide rows: 146 us, stored 64 bytes of a row at a time 239.)
 template <class TOut>
 constexpr int kBoxColumns = 128 / (int)sizeof(TOut);
 template <class TOut>
@@ -414,11 +415,13 @@ __device__ __forceinline__ void box_store(const CUtensorMap* map, const uint8_t*
 }
 __device__ __forceinline__ void box_stores_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }  // they have left shared memory
 __device__ __forceinline__ void box_stores_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+// Barriers of two warps (1 to 4) and of the four of a part of the columns (5, 6).
 __device__ __forceinline__ void two_warps_sync(int which) { asm volatile("bar.sync %0, 64;" ::"r"(1 + which) : "memory"); }
-// Whether any of two warps' threads says so: they meet at barriers of their own from here on, so they go on or end together.
-__device__ __forceinline__ bool two_warps_any(int which, bool mine) {
+__device__ __forceinline__ void four_warps_sync(int which) { asm volatile("bar.sync %0, 128;" ::"r"(5 + which) : "memory"); }
+// Whether any of four warps' threads says so: they meet at barriers of their own from here on, so they go on or end together.
+__device__ __forceinline__ bool four_warps_any(int which, bool mine) {
     uint32_t any;
-    asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 p, %2, 0;\nbar.red.or.pred q, %1, 64, p;\nselp.u32 %0, 1, 0, q;\n}" : "=r"(any) : "r"(1 + which), "r"((uint32_t)mine) : "memory");
+    asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 p, %2, 0;\nbar.red.or.pred q, %1, 128, p;\nselp.u32 %0, 1, 0, q;\n}" : "=r"(any) : "r"(5 + which), "r"((uint32_t)mine) : "memory");
     return any != 0;
 }
 // 16 lanes by 32 columns of TMEM, a fragment of 8 x 8 for each two registers: thread t has lane t / 4 (registers 0, 1 of four) or
@@ -510,6 +513,41 @@ __device__ __forceinline__ void store_columns(TOut* out, long long stride, const
 #pragma unroll
         for (int j = 0; j < ROWS; ++j)
             if (j < rows) lp::store_rounded(out + j * stride, acc[j]);
+    }
+}
+
+// Rows [first, end) of two boxes side by side, `live` columns of them, to rows of `out` that begin inside a 16-byte vector or a word: words
+// where they are whole, the columns at the ends alone.  (512 x 500 001 bf16 results of 256-wide rows: 211 us, and 288 stored 64 bytes of a
+// row at a time, where two of three sectors are written in part.  The eight rows are unrolled: with a test for each, 510.)
+template <class TOut>
+__device__ __forceinline__ void store_rows(const uint8_t* box, TOut* out, long long stride, int first, int end, int live) {
+    const int lane = threadIdx.x & 31;
+    const uint32_t mine = (uint32_t)(lane * 4);  // two columns of each box; its 16 bytes are where the row's number moves them
+    if (live == kTileN && end - first == 8) {
+        uint16_t* to = reinterpret_cast<uint16_t*>(out + first * stride);
+#pragma unroll
+        for (int r = 0; r < 8; ++r, to += stride) {
+            const uint8_t* const at = box + first * 128 + r * 128 + (mine ^ (uint32_t)(r << 4));
+            const uint32_t a = *reinterpret_cast<const uint32_t*>(at), b = *reinterpret_cast<const uint32_t*>(at + 4096);
+            if ((reinterpret_cast<uintptr_t>(to) & 2u) == 0) {
+                uint32_t* const words = reinterpret_cast<uint32_t*>(to) + lane;
+                words[0] = a, words[32] = b;
+            } else {  // a word takes its lower half from the columns before
+                const uint32_t before_a = __shfl_up_sync(~0u, a, 1), last_a = __shfl_sync(~0u, a, 31);
+                uint32_t before_b = __shfl_up_sync(~0u, b, 1);
+                if (lane == 0) before_b = last_a;
+                uint32_t* const words = reinterpret_cast<uint32_t*>(to - 1) + lane;
+                if (lane > 0) words[0] = __funnelshift_r(before_a, a, 16);
+                else to[0] = (uint16_t)a;
+                words[32] = __funnelshift_r(before_b, b, 16);
+                if (lane == 31) to[kTileN - 1] = (uint16_t)(b >> 16);
+            }
+        }
+    } else {
+        for (int row = first; row < end; ++row)
+            for (int c = lane; c < live; c += 32)
+                reinterpret_cast<uint16_t*>(out + row * stride)[c] =
+                    *reinterpret_cast<const uint16_t*>(box + c / 64 * 4096 + row * 128 + ((c % 64 / 8 ^ (row & 7)) << 4) + c % 8 * 2);
     }
 }
 
@@ -635,31 +673,23 @@ k_product8(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CU
         uint32_t parity = 0;
         if constexpr (RESIDENT) {
             constexpr int kRows = L::kWarpColumns < 32 ? L::kWarpColumns : 32, kChunks = L::kWarpColumns / kRows;
-            constexpr bool kStage = TM >= 64, kWide = sizeof(TOut) == 4;  // fp32 boxes are one warp's
+            // 16-bit results are turned, two warps' into a box; fp32 boxes are one warp's
+            constexpr bool kWide = sizeof(TOut) == 4, kTurn = TM >= 64 && !kWide;
             uint8_t* const box = boxes + pair * L::kBoxBytes + (kWide ? quad % 2 * (L::kBoxBytes / 2) : 0);
             const bool issues = lane == 0 && (kWide || quad % 2 == 0);
-            const bool fragments = kStage && !kWide && g.staged;
             for (Tiles<RESIDENT> tile(g); tile.here(g); tile.w += tile.step) {
                 const int n0 = tile.nt * kTileN + quad * 32, m0 = tile.mt * TM + column0;
                 float acc[kChunks][32];  // 32 columns each, a lane's or (to be turned) two fragments of 16 lanes
                 bool ended = false;
                 for (int kb = 0; kb < g.blocks; kb += kSegment) {
-                    if (two_warps_any(pair, !wait(&s_done[slot], parity, gave_up))) {
+                    if (four_warps_any(part, !wait(&s_done[slot], parity, gave_up))) {
                         ended = true;
                         break;
                     }
                     tc::tc_fence_after();
-                    // of shared columns those that read them, the last 64 of slot 0 and the first 64 of slot 1, hold up the next tile
-                    const bool holds = !L::kShare || part == (slot == 0 ? L::kColumnWarps - 1 : 0);
-                    const auto release = [&] {
-                        tc::tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) tc::mbar_arrive(&s_free[L::kShare ? 0 : slot]);
-                    };
-                    if (!holds) release();
                     const uint32_t taddr = tmem + slot * L::kNextColumns + column0 + ((uint32_t)(quad * 32) << 16);
                     uint32_t sum[kChunks][32];
-                    if (fragments) {
+                    if constexpr (kTurn) {
                         uint32_t lo[kChunks][16], hi[kChunks][16];
 #pragma unroll
                         for (int i = 0; i < kChunks; ++i) tmem_ld_fragments(taddr + 32 * i, lo[i]), tmem_ld_fragments(taddr + 32 * i + (16u << 16), hi[i]);
@@ -672,7 +702,9 @@ k_product8(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CU
 #pragma unroll
                         for (int i = 0; i < kChunks; ++i) tc::tmem_ld32(taddr + 32 * i, sum[i]);
                     }
-                    if (holds) release();
+                    tc::tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive(&s_free[slot]);
 #pragma unroll
                     for (int i = 0; i < kChunks; ++i)
 #pragma unroll
@@ -685,41 +717,49 @@ k_product8(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CU
 #pragma unroll
                 for (int i = 0; i < kChunks; ++i) {
                     const int rows = min(kRows, g.m - m0 - 32 * i);
-                    if (rows <= 0) break;  // the same for both warps
-                    if (kStage && g.staged) {
-                        if constexpr (kStage && !kWide) {
+                    if (rows <= 0) break;  // the same for the four warps
+                    if constexpr (kTurn) {
+                        if (g.boxes) {
                             if (issues) box_stores_read();
                             two_warps_sync(pair);
+                        } else {
+                            four_warps_sync(part);  // the rows before have been read
+                        }
 #pragma unroll
-                            for (int q = 0; q < 4; ++q) {  // eight rows of `out` each, of 16 bytes for each eight lanes
-                                const uint32_t at = tc::smem_u32(box) + (q * 8 + (lane & 7)) * 128 + (((quad % 2 * 4 + lane / 8) ^ (lane & 7)) << 4);
-                                const float* const lo = acc[i] + 4 * q;
-                                const float* const hi = acc[i] + 16 + 4 * q;
-                                store_turned(at, rounded_pair<TOut>(lo[0], lo[1]), rounded_pair<TOut>(lo[2], lo[3]), rounded_pair<TOut>(hi[0], hi[1]), rounded_pair<TOut>(hi[2], hi[3]));
-                            }
+                        for (int q = 0; q < 4; ++q) {  // eight rows of `out` each, of 16 bytes for each eight lanes
+                            const uint32_t at = tc::smem_u32(box) + (q * 8 + (lane & 7)) * 128 + (((quad % 2 * 4 + lane / 8) ^ (lane & 7)) << 4);
+                            const float* const lo = acc[i] + 4 * q;
+                            const float* const hi = acc[i] + 16 + 4 * q;
+                            store_turned(at, rounded_pair<TOut>(lo[0], lo[1]), rounded_pair<TOut>(lo[2], lo[3]), rounded_pair<TOut>(hi[0], hi[1]), rounded_pair<TOut>(hi[2], hi[3]));
+                        }
+                        if (g.boxes) {
                             tc::fence_async_shared();
                             two_warps_sync(pair);
                             if (issues && n0 < g.n) box_store(&out_map, box, n0, m0 + 32 * i);
-                        } else if constexpr (kStage) {
+                        } else {
+                            four_warps_sync(part);
+                            store_rows(boxes + part * 2 * L::kBoxBytes, static_cast<TOut*>(g.out) + (long long)(m0 + 32 * i) * g.out_stride + tile.nt * kTileN, g.out_stride,
+                                       quad * 8, min(rows, quad * 8 + 8), min(kTileN, g.n - tile.nt * kTileN));
+                        }
+                    } else if (TM >= 64 && g.boxes) {
 #pragma unroll
-                            for (int h = 0; h < 32; h += kBoxRows<TOut>) {
-                                if (h >= rows) break;
-                                if (issues) box_stores_read();
-                                __syncwarp();
-                                TOut* const to = reinterpret_cast<TOut*>(box) + lane;
+                        for (int h = 0; h < 32; h += kBoxRows<TOut>) {
+                            if (h >= rows) break;
+                            if (issues) box_stores_read();
+                            __syncwarp();
+                            TOut* const to = reinterpret_cast<TOut*>(box) + lane;
 #pragma unroll
-                                for (int q = 0; q < kBoxRows<TOut>; ++q) lp::store_rounded(to + q * 32, acc[i][(h + q) % 32]);
-                                tc::fence_async_shared();
-                                __syncwarp();
-                                if (issues && n0 < g.n) box_store(&out_map, box, n0, m0 + 32 * i + h);
-                            }
+                            for (int q = 0; q < kBoxRows<TOut>; ++q) lp::store_rounded(to + q * 32, acc[i][(h + q) % 32]);
+                            tc::fence_async_shared();
+                            __syncwarp();
+                            if (issues && n0 < g.n) box_store(&out_map, box, n0, m0 + 32 * i + h);
                         }
                     } else {
                         store_columns<kRows>(out + (long long)(32 * i) * g.out_stride, g.out_stride, acc[i], n0 + lane < g.n ? rows : 0);
                     }
                 }
             }
-            if (kStage && g.staged && issues) box_stores_done();
+            if (TM >= 64 && g.boxes && issues) box_stores_done();
         } else {
             // the columns in halves; the upper warps begin with their second one, which is where columns are shared
             constexpr int kHalf = L::kWarpColumns / 2;

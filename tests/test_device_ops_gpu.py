@@ -354,11 +354,14 @@ def test_product8(ops, m, n, k):
         got = ops.product8(a, b, dtype=out).cpu().double()
         fine = want.abs() < 60000 if out == torch.float16 else torch.ones_like(want, dtype=torch.bool)
         assert torch.all(((got - want).abs() <= tol)[fine]), (out, ((got - want).abs() / tol)[fine].max())
-    frame = torch.full((m, n + 7), 5.0).cuda()
-    ops.product8(x.cuda(), b, out=frame[:, 3 : n + 3])
-    want, tol = product_tolerance(forms.rows8(x)[0], forms.rows8(y)[0], k, torch.float32)
-    assert torch.all((frame[:, 3 : n + 3].cpu().double() - want).abs() <= tol)
-    assert torch.all(frame[:, :3] == 5) and torch.all(frame[:, n + 3 :] == 5)
+    for out in TYPES:  # into a part of a larger matrix, at every alignment
+        want, tol = product_tolerance(forms.rows8(x)[0], forms.rows8(y)[0], k, out)
+        fine = want.abs() < 60000 if out == torch.float16 else torch.ones_like(want, dtype=torch.bool)
+        for lead in (0, 3, 4):
+            frame = torch.full((m, n + 9 - lead % 2), 5.0, dtype=out).cuda()
+            ops.product8(x.cuda(), b, out=frame[:, lead : n + lead])
+            assert torch.all(((frame[:, lead : n + lead].cpu().double() - want).abs() <= tol)[fine])
+            assert torch.all(frame[:, :lead] == 5) and torch.all(frame[:, n + lead :] == 5)
     from distributed_kge_poplar_b200 import capi
 
     assert capi.load_library().kge_op_product8_status() == capi.OK
