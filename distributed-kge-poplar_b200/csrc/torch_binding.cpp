@@ -238,12 +238,13 @@ Tensor product8(const Rows8& a, const Rows8& b, at::ScalarType dtype, const Opti
 struct AdamWTensors {
     std::vector<Tensor> params;
     std::vector<kge_adamw_tensor> table;
-    std::vector<int64_t> first;
+    std::vector<int64_t> first, sizes;
+    at::ScalarType type;
     int64_t total = 0;
 
     explicit AdamWTensors(std::vector<Tensor> given) : params(std::move(given)) {
         if (params.empty()) refuse("AdamW needs at least one tensor");
-        const auto type = params[0].scalar_type();
+        type = params[0].scalar_type();
         std::vector<std::tuple<uintptr_t, uintptr_t, size_t>> spans;
         for (size_t i = 0; i < params.size(); ++i) {
             const Tensor& p = params[i];
@@ -260,6 +261,7 @@ struct AdamWTensors {
             }
             table.push_back(kge_adamw_tensor{nullptr, nullptr, 0, (size_t)total});
             first.push_back(total);
+            sizes.push_back(p.numel());
             total += (p.numel() + 127) / 128 * 128;
         }
         std::sort(spans.begin(), spans.end());
@@ -271,17 +273,31 @@ struct AdamWTensors {
               const OptionalTensor& v_exponent, double beta_m, double beta_v, double epsilon, double grad_scale, double decay, double step_size,
               double inv_sqrt_correction, uint32_t key, const OptionalTensor& schedule) {
         if (grads.size() != params.size()) refuse(grads.size(), " gradients for ", params.size(), " parameters");
-        const c10::Device device = params[0].device();
-        std::optional<at::ScalarType> type;
+        const c10::Device device = adam_m.device();
+        const auto must_be_moments = [&](const char* what, const Tensor& t, at::ScalarType kind, int64_t size) {
+            must_be_with(what, t, device);
+            if (t.scalar_type() != kind) refuse(what, " must be ", type_name(kind), ", not ", type_name(t.scalar_type()));
+            must_have_shape(what, t, {size});
+            if (!t.is_contiguous()) refuse(what, " must be contiguous");
+        };
+        must_be_moments("adam_m", adam_m, state_bits == 8 ? at::kByte : at::kFloat, total);
+        must_be_moments("adam_v", adam_v, state_bits == 8 ? at::kByte : at::kFloat, total);
+        if (state_bits == 8 && !(m_exponent && v_exponent)) refuse("moments in 8 bits have exponents");
+        if (m_exponent) must_be_moments("m_exponent", *m_exponent, at::kByte, total / 128);
+        if (v_exponent) must_be_moments("v_exponent", *v_exponent, at::kByte, total / 128);
+        std::optional<at::ScalarType> grad_type;
         for (size_t i = 0; i < grads.size(); ++i) {
             table[i].size = 0;
             if (!grads[i]) continue;
             const Tensor &g = *grads[i], &p = params[i];
-            if (!type) {
+            // what a tensor holds may have been replaced since the optimiser was made
+            if (p.device() != device || p.scalar_type() != type || p.numel() != sizes[i] || !p.is_contiguous())
+                refuse("parameter ", i, " is no longer ", sizes[i], " contiguous values of ", type_name(type), " on ", device);
+            if (!grad_type) {
                 must_be_float("gradients", g.scalar_type());
-                type = g.scalar_type();
+                grad_type = g.scalar_type();
             }
-            if (g.scalar_type() != *type) refuse("gradient ", i, " is ", type_name(g.scalar_type()), ", others ", type_name(*type));
+            if (g.scalar_type() != *grad_type) refuse("gradient ", i, " is ", type_name(g.scalar_type()), ", others ", type_name(*grad_type));
             if (g.device() != device) refuse("gradient ", i, " is on ", g.device(), ", the parameters on ", device);
             if (g.sizes() != p.sizes()) refuse("gradient ", i, " has shape ", g.sizes(), ", its parameter ", p.sizes());
             if (!g.is_contiguous()) refuse("gradient ", i, " must be contiguous");
@@ -289,10 +305,10 @@ struct AdamWTensors {
             table[i].grad = g.data_ptr();
             table[i].size = (size_t)p.numel();
         }
-        if (!type) return;
+        if (!grad_type) return;
         kge_adamw_args a{};
-        a.param_type = float_type(params[0].scalar_type());
-        a.grad_type = float_type(*type);
+        a.param_type = float_type(type);
+        a.grad_type = float_type(*grad_type);
         a.state_bits = state_bits;
         a.adam_m = adam_m.data_ptr();
         a.adam_v = adam_v.data_ptr();

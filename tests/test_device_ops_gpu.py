@@ -702,3 +702,23 @@ def test_gradients_that_are_broadcast_and_leaves_that_require_them(ops):
     before, version = leaf.detach().clone(), leaf._version
     optimiser.step([torch.ones_like(leaf)], 0.1)
     assert leaf._version > version and float((before - leaf.detach() - 0.1).abs().max()) < 1e-5
+
+
+def test_adamw_of_tensors_whose_memory_was_replaced(ops):
+    for change, text in [(lambda t: t.cpu(), "parameter 1 is no longer"), (lambda t: t.bfloat16(), "parameter 1 is no longer"), (lambda t: t.new_zeros(4, 300), "parameter 1 is no longer"),
+                         (lambda t: t.T.contiguous().T, "parameter 1 is no longer")]:
+        params = [torch.zeros(5).cuda(), torch.zeros(4, 3).cuda()]
+        optimiser = ops.AdamW(params)
+        params[1].data = change(params[1].data)
+        with pytest.raises(ValueError, match=text):
+            optimiser.step([torch.ones(5).cuda(), torch.ones_like(params[1])], 0.1)
+        assert torch.all(params[0] == 0)
+    optimiser = ops.AdamW([torch.zeros(400).cuda()], state_bits=8)
+    optimiser.adam_v = optimiser.adam_v[:128]
+    with pytest.raises(ValueError, match="adam_v has shape"):
+        optimiser.step([torch.ones(400).cuda()], 0.1)
+    params = [torch.zeros(4, 3).cuda()]
+    optimiser = ops.AdamW(params)
+    params[0].data = torch.ones(4, 3).cuda()
+    optimiser.step([torch.ones(4, 3).cuda()], 0.1)  # new memory of the same kind is updated
+    assert float((params[0] - 0.9).abs().max()) < 1e-5
