@@ -65,8 +65,10 @@ namespace {
 
 // A row is one block's, of as many threads as give each SM 1024: 128 rows of 100 003 bf16 scores with lists of 100 take 16 us by blocks
 // of 1024 threads, and in parts of 256 with a second kernel to join them 29.  Rows are cut into parts, four to an SM, where there are too
-// few of them for that or their groups of vectors do not fit a block's shared memory; two to an SM with lists, which each part makes (4
-// rows of 2 500 001 fp32 scores 24.6 us, with four to an SM 26.0, by one block a row 713).
+// few of them for that or the groups of vectors of their lists do not fit a block's shared memory; two to an SM with lists, which each part
+// makes (4 rows of 2 500 001 fp32 scores 24.6 us, with four to an SM 26.0, by one block a row 713).  Many short rows go to blocks of 128
+// threads, whose sums are joined sooner: 4096 rows of 10 001 bf16 scores 26.8 us, by blocks of 256 33.1, with lists of 10 41.3 and 63.5;
+// 4096 of 20 001 fp32 ones, 5001 vectors each, take 62 us either way.
 struct LogProbsPlan {
     int threads, parts, vectors;
     size_t sums_bytes, bytes;
@@ -79,12 +81,12 @@ LogProbsPlan log_probs_plan(size_t rows, size_t cols, size_t n_best, size_t widt
         return (size_t)threads * groups * lp::kGroup;
     };
     size_t parts = 1;
-    if (all <= 512) {
+    if (all <= 512 || (rows >= 4 * kSmCount && all <= (n_best ? most(128) : 4096))) {
         p.threads = 128;
     } else {
         p.threads = rows <= kSmCount + 12 ? 1024 : rows <= 2 * kSmCount + 24 ? 512 : 256;
         while (p.threads > 256 && (size_t)p.threads * 2 > all) p.threads /= 2;  // two vectors a thread at least
-        if (all > most(p.threads) || (rows <= kSmCount / 2 && (all > 16384 || (rows <= 16 && all >= 2048)))) {
+        if ((n_best && all > most(p.threads)) || (rows <= kSmCount / 2 && (all > 16384 || (rows <= 16 && all >= 2048)))) {
             p.threads = 256;
             parts = std::max((all + most(256) - 1) / most(256), std::min((n_best ? 2 : 4) * kSmCount / std::max<size_t>(1, rows), all / 1024));
         }

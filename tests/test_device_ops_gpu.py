@@ -69,7 +69,8 @@ def check_log_probs(got, want, cols, entropy_scale=1.0):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows,cols,n_best", [(1, 1, 1), (3, 1, 4), (2, 7, 10), (5, 63, 5), (1, 1387, 10), (4, 2049, 128), (7, 4097, 100), (2, 40_003, 17), (3, 100_001, 128),
-                                              (40, 20_001, 30), (20, 90_003, 100), (200, 9000, 100), (400, 5000, 128)])
+                                              (40, 20_001, 30), (20, 90_003, 100), (200, 9000, 100), (400, 5000, 128),
+                                              (600, 4003, 128), (600, 8003, 5), (592, 12_001, 0), (100, 140_001, 0)])
 def test_log_probs(ops, rows, cols, n_best, dtype):
     g = gen(rows * 1000 + cols)
     x = (torch.randn(rows, cols, generator=g) * 3).to(dtype)
