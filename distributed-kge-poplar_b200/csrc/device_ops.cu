@@ -188,7 +188,7 @@ void quantise_rows(const void* x, int float_type, size_t rows, size_t cols, long
         using T = decltype(t);
         const T* const src = static_cast<const T*>(x);
         if (!transposed) {
-            const size_t blocks = rows8::blocks_of(cols), units = round_up(rows, 128) * blocks, per = 8 * 4 * rows8::kUnits;
+            const size_t blocks = rows8::blocks_of(cols), units = round_up(rows, 128) * blocks, per = 8 * 4;
             if (units > 0xffffff00u) fail(KGE_INVALID_ARGUMENT, msg() << what << ": " << rows << " x " << cols << " is too large for one launch");
             const cudaError_t err = launch_dependent(rows8::k_quantise_rows<T>, dim3((unsigned)((units + per - 1) / per)), dim3(256), 0, stream, src, (uint32_t)rows, cols,
                                                      row_stride, (uint32_t)blocks, (uint32_t)rows8::groups_of(cols), (uint32_t)units, values, exponents);

@@ -53,19 +53,18 @@ __device__ __forceinline__ uint32_t to_e4m3x2(float lo, float hi) {
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(w) : "f"(hi), "f"(lo));
     return w;
 }
-// Sixteen values times `inverse` as e4m3.  The conversion saturates an infinity, so where some value is not finite (`special`) those
-// become NaN one by one.
-__device__ __forceinline__ uint4 to_e4m3x16(const float (&v)[16], float inverse, bool special) {
-    uint32_t w[4];
+// Values times `inverse` as e4m3, four to a word.  The conversion saturates an infinity, so where some value is not finite (`special`)
+// those become NaN one by one.
+template <int N>
+__device__ __forceinline__ void to_e4m3(const float (&v)[N], float inverse, bool special, uint32_t (&w)[N / 4]) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
+    for (int q = 0; q < N / 4; ++q)
         w[q] = to_e4m3x2(v[4 * q] * inverse, v[4 * q + 1] * inverse) | to_e4m3x2(v[4 * q + 2] * inverse, v[4 * q + 3] * inverse) << 16;
     if (special) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
+        for (int i = 0; i < N; ++i)
             if ((__float_as_uint(v[i]) & 0x7f800000u) == 0x7f800000u) w[i / 4] = (w[i / 4] & ~(0xffu << (8 * (i % 4)))) | (uint32_t)kNan << (8 * (i % 4));
     }
-    return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // Sixteen values as they lie in memory: 8 words of two or 16 of one.
@@ -142,57 +141,53 @@ struct Sixteen {
     }
 };
 
-// Eight lanes take a block, 16 consecutive values each, and a warp kUnits times four blocks, all fetched before the first is worked
-// on: bound by memory, it needs that much in flight.
-constexpr int kUnits = 4;
+// Eight lanes take a block, 16 consecutive values each.  Bound by memory: what is in flight is as many warps as fit (512 x 100 001 bf16
+// values 30.8 us, 5.0 TB/s, fp32 41.1 us, 6.2 TB/s; with four blocks' worth to each lane, all fetched first, but a third of the warps
+// 39.0 and 65.2).
 template <class T>
 static __global__ void __launch_bounds__(256) k_quantise_rows(const T* __restrict__ x, uint32_t rows, size_t cols, long long stride, uint32_t blocks, uint32_t groups,
                                                               uint32_t units, uint8_t* __restrict__ values, uint8_t* __restrict__ exponents) {
     grid_dependency_sync();
     const int lane = threadIdx.x & 31;
     const size_t ld = value_stride(cols);
-    const uint32_t unit0 = (blockIdx.x * 8 + threadIdx.x / 32) * (4 * kUnits) + lane / 8;  // (row, block), rows rounded up to 128
-    const T* const end = x + (long long)(rows - 1) * stride + (long long)cols;
-    Sixteen<T> raw[kUnits];
+    const uint32_t unit = (blockIdx.x * 8 + threadIdx.x / 32) * 4 + lane / 8, r = unit / blocks, block = unit - r * blocks;  // rows rounded up to 128
+    const size_t c0 = (size_t)block * kBlock + (lane & 7) * 16;
+    Sixteen<T> raw;
+    if (unit < units && r < rows && c0 < cols)
+        raw.load(x + (long long)r * stride + c0, (int)min((size_t)16, cols - c0), x, x + (long long)(rows - 1) * stride + (long long)cols);
+    else raw.clear();
+    float v[16];
+    raw.floats(v);
+    uint32_t largest = raw.largest();
 #pragma unroll
-    for (int u = 0; u < kUnits; ++u) {
-        const uint32_t unit = unit0 + 4 * u, r = unit / blocks, block = unit - r * blocks;
-        const size_t c0 = (size_t)block * kBlock + (lane & 7) * 16;
-        if (unit < units && r < rows && c0 < cols) raw[u].load(x + (long long)r * stride + c0, (int)min((size_t)16, cols - c0), x, end);
-        else raw[u].clear();
+    for (int o = 4; o > 0; o >>= 1) largest = max(largest, __shfl_xor_sync(~0u, largest, o));
+    const bool special = largest >= 0x7f800000u;
+    if (__any_sync(~0u, special)) {
+        uint32_t finite = 0;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) finite = max(finite, finite_magnitude(v[j]));
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) finite = max(finite, __shfl_xor_sync(~0u, finite, o));
+        largest = finite;
     }
-#pragma unroll
-    for (int u = 0; u < kUnits; ++u) {
-        const uint32_t unit = unit0 + 4 * u, r = unit / blocks, block = unit - r * blocks;
-        float v[16];
-        raw[u].floats(v);
-        uint32_t largest = raw[u].largest();
-#pragma unroll
-        for (int o = 4; o > 0; o >>= 1) largest = max(largest, __shfl_xor_sync(~0u, largest, o));
-        const bool special = largest >= 0x7f800000u;
-        if (__any_sync(~0u, special)) {
-            uint32_t finite = 0;
-#pragma unroll
-            for (int j = 0; j < 16; ++j) finite = max(finite, finite_magnitude(v[j]));
-#pragma unroll
-            for (int o = 4; o > 0; o >>= 1) finite = max(finite, __shfl_xor_sync(~0u, finite, o));
-            largest = finite;
-        }
-        if (unit >= units) continue;
-        const int byte = exponent_byte(largest);
-        if ((lane & 7) == 0) {
-            uint8_t* const bytes = exponents + (size_t)(r / 128) * groups * kGroupBytes + (r % 32) * 16 + (r % 128) / 32 * 4;
-            bytes[block / 4 * kGroupBytes + block % 4] = (uint8_t)byte;
-            for (uint32_t none = block + 1; block + 1 == blocks && none % 4 != 0; ++none) bytes[none / 4 * kGroupBytes + none % 4] = kOne;
-        }
-        const size_t c0 = (size_t)block * kBlock + (lane & 7) * 16;
-        if (r < rows && c0 < ld) *reinterpret_cast<uint4*>(values + (size_t)r * ld + c0) = to_e4m3x16(v, inverse_scale(byte), special);
+    if (unit >= units) return;
+    const int byte = exponent_byte(largest);
+    if ((lane & 7) == 0) {
+        uint8_t* const bytes = exponents + (size_t)(r / 128) * groups * kGroupBytes + (r % 32) * 16 + (r % 128) / 32 * 4;
+        bytes[block / 4 * kGroupBytes + block % 4] = (uint8_t)byte;
+        for (uint32_t none = block + 1; block + 1 == blocks && none % 4 != 0; ++none) bytes[none / 4 * kGroupBytes + none % 4] = kOne;
+    }
+    if (r < rows && c0 < ld) {
+        uint32_t w[4];
+        to_e4m3(v, inverse_scale(byte), special, w);
+        *reinterpret_cast<uint4*>(values + (size_t)r * ld + c0) = make_uint4(w[0], w[1], w[2], w[3]);
     }
 }
 
 // The columns of x as rows: a block is 128 rows of x in one column.  64 columns and 128 rows to a thread block; a warp takes 16 rows,
 // a thread two columns of them: neighbours where two fit a word, so that a warp reads 128 bytes of a row at once (value by value
-// 512 x 100 001 bf16 values took 96 us, this 45).  The bytes are turned in shared memory and written 128 side by side.
+// 512 x 100 001 bf16 values took 96 us, this 39.1; by warps of eight rows, twice as many, 52.7; 256 bytes of a row
+// to a block 42.7).  The bytes are turned in shared memory and written 128 side by side.
 constexpr int kTurnCols = 64;
 template <class T>
 static __global__ void __launch_bounds__(256) k_quantise_columns(const T* __restrict__ x, size_t rows, size_t cols, long long stride, size_t groups,
@@ -203,7 +198,7 @@ static __global__ void __launch_bounds__(256) k_quantise_columns(const T* __rest
     __shared__ alignas(16) uint8_t s_out[kTurnCols * kPitch];
     grid_dependency_sync();
     const size_t blocks = (rows + kBlock - 1) / kBlock;
-    const size_t tiles = (cols + 127) / 128 * (128 / kTurnCols);  // columns are rounded up to 128
+    const uint32_t tiles = (uint32_t)((cols + 127) / 128 * (128 / kTurnCols));  // columns are rounded up to 128
     const size_t block = blockIdx.x / tiles, tile = blockIdx.x % tiles;  // neighbours read neighbouring parts of the same rows
     const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
     const size_t c0 = tile * kTurnCols, r0 = block * kBlock + (size_t)warp * 16, ld = value_stride(rows);
@@ -290,7 +285,9 @@ static __global__ void __launch_bounds__(256) k_quantise_columns(const T* __rest
         if (warp == 0) exponents[((c / 128) * groups + block / 4) * kGroupBytes + (c % 32) * 16 + (c % 128) / 32 * 4 + block % 4] = (uint8_t)byte;
         float v[16];
         column(h, v);
-        *reinterpret_cast<uint4*>(s_out + own[h] * kPitch + warp * 16) = to_e4m3x16(v, inverse_scale(byte), special[h]);
+        uint32_t e[4];
+        to_e4m3(v, inverse_scale(byte), special[h], e);
+        *reinterpret_cast<uint4*>(s_out + own[h] * kPitch + warp * 16) = make_uint4(e[0], e[1], e[2], e[3]);
     }
     __syncthreads();
 #pragma unroll
