@@ -816,9 +816,11 @@ constexpr int kGradThreads = 256;
 
 // One block for kGradThreads * kGroup vectors of a row, the rows from the last to the first: what the forward pass read last may
 // still be in L2.  The vectors are those of the scores' memory: a gradient that is as far from a 16-byte boundary as the scores
-// are is written as it is read.
+// are is written as it is read.  Bound by memory, it takes 144 us of 2048 x 100 001 bf16 scores and 156 of half as many fp32 ones (127 at
+// the copy rate); with registers for four blocks an SM 153 and 172, with two vectors a thread 164, for six blocks and a few spills 141
+// and 162.
 template <class T>
-static __global__ void __launch_bounds__(kGradThreads, 4) k_log_probs_grad(Scores s, GradArgs g) {
+static __global__ void __launch_bounds__(kGradThreads, 5) k_log_probs_grad(Scores s, GradArgs g) {
     constexpr int V = Row<T>::V;
     __shared__ float s_sum;
     __shared__ float s_best[kMaxBest];
