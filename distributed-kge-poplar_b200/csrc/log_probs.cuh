@@ -564,6 +564,7 @@ template <int THREADS>
 __device__ __forceinline__ void thin_candidates(int n_best, Shared<THREADS>& sh) {
     const int n = sh.count;
     if (n <= 2 * kMaxBest || n > kCandidates) return;
+    __syncthreads();  // every thread has read the count, and the caller's tests of it are done: first_threshold sets it to 0
     constexpr int kPer = kCandidates / THREADS;
     unsigned long long key[kPer];
     uint32_t largest = 0;

@@ -1,0 +1,124 @@
+"""The operators on device tensors where their definitions are easily missed: values that are not finite or far from the others, lists
+that are thinned out, larger blocks, tiles and parts."""
+
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+import device_op_forms as forms  # noqa: E402
+from test_device_ops_gpu import TYPES, U, check_log_probs, cuda, gen, grad_tolerance, log_tolerance, ops  # noqa: E402, F401
+
+pytestmark = pytest.mark.gpu
+
+# Rows and columns of fp32 scores for which a row is one block of 128, 256, 512 or 1024 threads, or is cut into parts.
+SHAPES = {128: (6, 1500), 256: (330, 9001), 512: (200, 9001), 1024: (100, 20_001), "few parts": (1, 100_001), "parts": (3, 150_001)}
+
+
+@pytest.mark.parametrize("size", SHAPES)
+def test_lists_of_many_candidates(ops, size):  # noqa: F811
+    """600 columns share the best score: more pass the first threshold than are ranked, so a second one is looked for among them."""
+    rows, cols = SHAPES[size]
+    g = gen(cols)
+    x = torch.randn(rows, cols, generator=g).clamp(max=2.0)
+    at = torch.stack([torch.randperm(cols, generator=g)[:600] for _ in range(rows)])
+    x.scatter_(1, at, 3.0)
+    want = at.sort(1).values[:, :100].int()
+    device = x.cuda()
+    for _ in range(20):
+        got = ops.log_probs(device, n_best=100)
+        assert torch.equal(got.best_index.cpu(), want)
+    few = min(rows, 12)
+    check_log_probs(ops.log_probs(device[:few], n_best=100), forms.log_probs(x[:few], None, n_best=100), cols)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_live_nan_wherever_it_is(ops, dtype):  # noqa: F811
+    """Short rows at every alignment, the NaN in each of their columns: it may be all that a thread sees."""
+    for cols in range(1, 20):
+        for lead in range(8):
+            wide = torch.randn(cols, cols + 9, generator=gen(cols * 10 + lead)).to(dtype)
+            x = wide[:, lead : lead + cols]
+            x.diagonal().fill_(math.nan)
+            device = wide.cuda()[:, lead : lead + cols]
+            target = torch.zeros(cols, dtype=torch.int32)
+            got = ops.log_probs(device, target.cuda(), n_best=4)
+            check_log_probs(got, forms.log_probs(x, target, n_best=4), cols)
+            assert torch.all(torch.isnan(got.log_sum)) and torch.all(torch.isnan(got.entropy)) and torch.all(torch.isnan(got.log_prob))
+            assert torch.all(torch.isnan(ops.log_probs_grad(device, got, grad_log_prob=torch.ones(cols).cuda())))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hidden", ["mask", "-inf"])
+@pytest.mark.parametrize("size", SHAPES)
+def test_a_live_nan_among_hidden_columns(ops, size, hidden, dtype):  # noqa: F811
+    """One NaN and twenty other live columns a row, far apart; in every third row the NaN is hidden too."""
+    rows, cols = SHAPES[size]
+    g = gen(cols + 1)
+    x = torch.randn(rows, cols, generator=g).to(dtype)
+    at = torch.stack([torch.randperm(cols, generator=g)[:21] for _ in range(rows)])
+    live = torch.zeros(rows, cols, dtype=torch.bool).scatter_(1, at, True)
+    live[torch.arange(0, rows, 3), at[::3, 0]] = False
+    x[torch.arange(rows), at[:, 0]] = math.nan
+    target = at[:, 1].int().contiguous()
+    mask = live if hidden == "mask" else None
+    if hidden == "-inf":
+        x = torch.where(live, x, -math.inf)
+    got = ops.log_probs(x.cuda(), target.cuda(), mask=cuda(mask), n_best=25)
+    check_log_probs(got, forms.log_probs(x, target, mask, n_best=25), cols)
+    lost = torch.ones(rows, dtype=torch.bool)
+    lost[::3] = False
+    assert torch.equal(torch.isnan(got.log_sum).cpu(), lost)
+    grad = ops.log_probs_grad(x.cuda(), got, grad_log_prob=torch.ones(rows).cuda()).cpu()
+    assert torch.equal(torch.isnan(grad), live & lost[:, None]) and torch.all(grad[~live] == 0)
+
+
+@pytest.mark.parametrize("far", [-1e9, -3e9, -1e10, -1e20, 1e10, 1e20])
+@pytest.mark.parametrize("dtype,scale", [(torch.float32, 1.0), (torch.bfloat16, 0.5), (torch.float16, 1e6)])
+@pytest.mark.parametrize("cols", [5000, 70_001])
+def test_scores_far_from_the_others(ops, cols, dtype, scale, far):  # noqa: F811
+    """Finite numbers that stand for hidden columns, or for the one answer: logits whose rounding in fp32 is more than a power of two's
+    whole range.  A row's own differences are what counts; equal scores share the row however far out they are."""
+    far = max(-65504.0, min(65504.0, far / scale)) if dtype == torch.float16 else far
+    g = gen(cols)
+    x = (torch.randn(8, cols, generator=g) * (3 / max(scale, 1.0))).to(dtype)
+    x[0] = far
+    x[1, : cols // 2] = far
+    x[2, -40:] = far
+    x[3, : cols - cols // 10] = far
+    x[4] = far
+    x[4, cols - 1] = 1.0
+    x[5].view(-1, 8 if cols % 8 == 0 else 1)[::2] = far
+    x[6] = far
+    x[6, ::3] = -math.inf
+    x[7, 4] = far
+    target = torch.tensor([3, 5, cols - 1, cols - 2, cols - 1, 2, 1, 4], dtype=torch.int32)
+    weights = [torch.randn(shape, generator=g) / max(scale, 1.0) for shape in ((8,), (8,), (8, 5))]
+    want = forms.log_probs(x, target, scale=scale, n_best=5)
+    got = ops.log_probs(x.cuda(), target.cuda(), scale=scale, n_best=5)
+    for name in ("log_prob", "log_sum", "best_log_prob"):
+        a, b = getattr(got, name).cpu().double(), want[name]
+        assert torch.all((a - b).abs() <= log_tolerance(cols, b)), (name, a, b)
+    a, b = got.entropy.cpu().double(), want["entropy"]
+    assert torch.all((a - b).abs() <= log_tolerance(cols, b) * (1 + b))
+    assert torch.equal(got.best_index.cpu(), want["best_index"])
+    grad = ops.log_probs_grad(x.cuda(), got, grad_log_prob=weights[0].cuda(), grad_entropy=weights[1].cuda(), grad_best=weights[2].cuda()).cpu().double()
+    right = forms.log_probs_grad(x, want, target, scale, *weights)
+    total = weights[0].double().abs() + weights[2].double().abs().sum(1)
+    tol = grad_tolerance(want, dtype, total, weights[1].double(), scale, cols, right)
+    assert torch.all((grad - right).abs() <= tol), ((grad - right).abs() / tol).max()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_of_tiny_gradients(ops, bits):  # noqa: F811
+    """Second moments that are subnormal in fp32 count: (1 - beta_v) g^2 and its sum are off by a step of subnormal numbers, 2^-149, which
+    moves the root by that over 2 v of itself.  A step in 8 bits divides by the sum before it is encoded."""
+    g = torch.exp(torch.linspace(math.log(2e-20), math.log(3e-16), 4096).double()).float() * torch.tensor([1.0, -1.0]).repeat(2048)
+    p = torch.zeros(4096).cuda()
+    optimiser = ops.AdamW([p], state_bits=bits, beta_m=0.9, beta_v=0.999, epsilon=1e-20)
+    optimiser.step([g.cuda()], 0.01)
+    m, v = 0.1 * g.double(), 0.001 * g.double() ** 2
+    want = -0.01 * (m / 0.1) / ((v / 0.001).sqrt() + 1e-20)
+    off = 2.0**-149 / (2 * v) + 32 * U
+    assert torch.all((p.cpu().double() - want).abs() <= off * want.abs())
