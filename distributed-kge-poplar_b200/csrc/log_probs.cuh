@@ -672,8 +672,12 @@ __device__ __forceinline__ Sums add_part(const Row<T>& row, int v0, int v1, floa
 #pragma unroll
         for (int u = 0; u < kGroup; ++u) raw[u] = next[u];
     }
-    if (reference == W::kLow) return Sums{reference, 0.f, 0.f};
-    const float off = fmaf(reference, s2, -r2), c = ex2(-off), total = halves(sum).x + halves(sum).y;
+    const float total = halves(sum).x + halves(sum).y;
+    if (reference == W::kLow) {  // nothing counts but a NaN, which has not moved the reference
+        const float nan = total == total ? 0.f : total;
+        return Sums{reference, nan, nan};
+    }
+    const float off = fmaf(reference, s2, -r2), c = ex2(-off);
     return Sums{reference, c * total, c * fmaf(-off, total, halves(weighted).x + halves(weighted).y)};
 }
 template <int THREADS, class T>

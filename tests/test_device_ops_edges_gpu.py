@@ -1,12 +1,14 @@
 """The operators on device tensors where their definitions are easily missed: values that are not finite or far from the others, lists
 that are thinned out, larger blocks, tiles and parts."""
 
+import math
+
 import pytest
 
 torch = pytest.importorskip("torch")
 
 import device_op_forms as forms  # noqa: E402
-from test_device_ops_gpu import check_log_probs, gen, ops  # noqa: E402, F401
+from test_device_ops_gpu import TYPES, check_log_probs, cuda, gen, ops  # noqa: E402, F401
 
 pytestmark = pytest.mark.gpu
 
@@ -29,3 +31,44 @@ def test_lists_of_many_candidates(ops, size):  # noqa: F811
         assert torch.equal(got.best_index.cpu(), want)
     few = min(rows, 12)
     check_log_probs(ops.log_probs(device[:few], n_best=100), forms.log_probs(x[:few], None, n_best=100), cols)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_live_nan_wherever_it_is(ops, dtype):  # noqa: F811
+    """Short rows at every alignment, the NaN in each of their columns: it may be all that a thread sees."""
+    for cols in range(1, 20):
+        for lead in range(8):
+            wide = torch.randn(cols, cols + 9, generator=gen(cols * 10 + lead)).to(dtype)
+            x = wide[:, lead : lead + cols]
+            x.diagonal().fill_(math.nan)
+            device = wide.cuda()[:, lead : lead + cols]
+            target = torch.zeros(cols, dtype=torch.int32)
+            got = ops.log_probs(device, target.cuda(), n_best=4)
+            check_log_probs(got, forms.log_probs(x, target, n_best=4), cols)
+            assert torch.all(torch.isnan(got.log_sum)) and torch.all(torch.isnan(got.entropy)) and torch.all(torch.isnan(got.log_prob))
+            assert torch.all(torch.isnan(ops.log_probs_grad(device, got, grad_log_prob=torch.ones(cols).cuda())))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hidden", ["mask", "-inf"])
+@pytest.mark.parametrize("size", SHAPES)
+def test_a_live_nan_among_hidden_columns(ops, size, hidden, dtype):  # noqa: F811
+    """One NaN and twenty other live columns a row, far apart; in every third row the NaN is hidden too."""
+    rows, cols = SHAPES[size]
+    g = gen(cols + 1)
+    x = torch.randn(rows, cols, generator=g).to(dtype)
+    at = torch.stack([torch.randperm(cols, generator=g)[:21] for _ in range(rows)])
+    live = torch.zeros(rows, cols, dtype=torch.bool).scatter_(1, at, True)
+    live[torch.arange(0, rows, 3), at[::3, 0]] = False
+    x[torch.arange(rows), at[:, 0]] = math.nan
+    target = at[:, 1].int().contiguous()
+    mask = live if hidden == "mask" else None
+    if hidden == "-inf":
+        x = torch.where(live, x, -math.inf)
+    got = ops.log_probs(x.cuda(), target.cuda(), mask=cuda(mask), n_best=25)
+    check_log_probs(got, forms.log_probs(x, target, mask, n_best=25), cols)
+    lost = torch.ones(rows, dtype=torch.bool)
+    lost[::3] = False
+    assert torch.equal(torch.isnan(got.log_sum).cpu(), lost)
+    grad = ops.log_probs_grad(x.cuda(), got, grad_log_prob=torch.ones(rows).cuda()).cpu()
+    assert torch.equal(torch.isnan(grad), live & lost[:, None]) and torch.all(grad[~live] == 0)
