@@ -621,17 +621,18 @@ struct Parts {
 };
 
 // The sums of a part's vectors, four vectors a thread in flight at once and the next four while these are summed, in two halves:
-//   d = x s2 - r2 (one fused multiply-add), e = 2^d, sum += e, weighted += e d
-// with r2 the reference times s2, rounded: whatever it is off by, all terms are, and it is taken out exactly at the end.  Scores
-// are raised to kLow first, so that -inf makes no NaN of e d; where the largest score is no further than 2^64 above kLow that
-// would count them, and add_exactly does the part again.
+//   d = (x - reference) s2, e = 2^d, sum += e, weighted += e d
+// The difference is taken first: it is right, and never above 0, however far out the scores are.  (x s2 less the rounded product of the
+// reference is one instruction, and off by half a unit of that product: from 2^31 on more than fp32 has exponents for.)  Scores are
+// raised to kLow first, so that -inf makes no NaN of e d; where the largest score is no further than 2^64 above kLow that would count
+// them, and add_exactly does the part again.
 // Reading bounds fp32 rows (1024 x 200 001: 133 us, 6.1 TB/s); of bf16 ones, twice the scores for the same bytes, the exponentials, 16 an SM
 // and cycle, take 45 of 82 us beside the reading's 62 (2048 x 100 001: 5.0 TB/s; 83.5 without the next four vectors under way and one
 // sum at a time).
 template <int THREADS, class T>
 __device__ __forceinline__ Sums add_part(const Row<T>& row, int v0, int v1, float s2, float* groups, float& largest) {
     using W = Words<T>;
-    float reference = W::kLow, r2 = 0.f;  // until a score is above kLow nothing counts
+    float reference = W::kLow;  // until a score is above kLow nothing counts
     Pair sum = pair(0.f, 0.f), weighted = sum;
     const Pair scale = pair(s2, s2);
     int at = threadIdx.x & 31;
@@ -651,19 +652,18 @@ __device__ __forceinline__ Sums add_part(const Row<T>& row, int v0, int v1, floa
         largest = fmaxf(largest, above);
         if (groups) groups[at] = above;
         if (above > reference) {
-            reference = above;
-            const float to = above * s2, d = fminf(fmaxf(r2 - to, kFarBelow), 0.f), c = ex2(d);
+            const float d = fmaxf((reference - above) * s2, kFarBelow), c = ex2(d);
             weighted = mul_pair(pair(c, c), fma_pair(sum, pair(d, d), weighted));
             sum = mul_pair(pair(c, c), sum);
-            r2 = to;
+            reference = above;
         }
-        const Pair back = pair(-r2, -r2);
+        const Pair back = pair(-reference, -reference);
 #pragma unroll
         for (int u = 0; u < kGroup; ++u)
 #pragma unroll
             for (int i = 0; i < 4; i += 3 - W::kPer) {
                 const float2 x = W::kPer == 2 ? W::floats(W::raised(raw[u].w[i])) : make_float2(W::floats(W::raised(raw[u].w[i])).x, W::floats(W::raised(raw[u].w[(i + 1) % 4])).x);
-                const Pair d = fma_pair(pair(x.x, x.y), scale, back);
+                const Pair d = mul_pair(add_pair(pair(x.x, x.y), back), scale);
                 const float2 power = halves(d);
                 const Pair e = pair(ex2(power.x), ex2(power.y));
                 sum = add_pair(sum, e);
@@ -677,8 +677,7 @@ __device__ __forceinline__ Sums add_part(const Row<T>& row, int v0, int v1, floa
         const float nan = total == total ? 0.f : total;
         return Sums{reference, nan, nan};
     }
-    const float off = fmaf(reference, s2, -r2), c = ex2(-off);
-    return Sums{reference, c * total, c * fmaf(-off, total, halves(weighted).x + halves(weighted).y)};
+    return Sums{reference, total, halves(weighted).x + halves(weighted).y};
 }
 template <int THREADS, class T>
 __device__ __noinline__ Sums add_exactly(const Row<T>& row, int v0, int v1, float s2) {
@@ -693,8 +692,10 @@ __device__ __noinline__ Sums add_exactly(const Row<T>& row, int v0, int v1, floa
     return sums;
 }
 
+// Blocks of 128 threads: eight to an SM, of fp32 scores seven, whose 72 registers hold both groups of vectors (600 x 5001: 6.2 us, with
+// eight 7.7; 1000 x 12 001: 11.6 and 14.6).
 template <class T, int THREADS>
-static __global__ void __launch_bounds__(THREADS, THREADS == 128 ? 8 : 1024 / THREADS) k_log_probs(Scores s, Out out, Parts parts) {
+static __global__ void __launch_bounds__(THREADS, THREADS == 128 ? (sizeof(T) == 4 ? 7 : 8) : 1024 / THREADS) k_log_probs(Scores s, Out out, Parts parts) {
     using W = Words<T>;
     __shared__ Shared<THREADS> sh;
     grid_dependency_sync();
@@ -872,14 +873,10 @@ static __global__ void __launch_bounds__(kGradThreads, 5) k_log_probs_grad(Score
         __syncthreads();
         total += s_sum;
     }
-    // -scale p (G + g_H (log p + entropy)) with log2 p = (x s2 - r2) - (log2 S + what r2 = reference s2 was rounded by); where the
-    // reference has no finite r2 (scores of the type's lowest value) from the difference of the scores
-    const float r2 = state.x * s.s2;
-    const bool usual = fabsf(r2) < 1e37f;
-    const float l2 = usual ? state.y + fmaf(state.x, s.s2, -r2) : state.y;
+    // -scale p (G + g_H (log p + entropy)) with log2 p = (x - reference) s2 - log2 S, the difference first as in the forward pass
     const float slope = -s.scale * g_entropy * kLn2, level = -s.scale * fmaf(g_entropy, state.z, total);
     auto gradient = [&](float x) {
-        const float d = max_or_nan((usual ? fmaf(x, s.s2, -r2) : (x - state.x) * s.s2) - l2, kFarBelow);
+        const float d = max_or_nan(fmaf(x - state.x, s.s2, -state.y), kFarBelow);
         return x == -INFINITY ? 0.f : ex2(d) * fmaf(slope, d, level);
     };
 #pragma unroll
@@ -889,19 +886,14 @@ static __global__ void __launch_bounds__(kGradThreads, 5) k_log_probs_grad(Score
         float val[V];
         unpack<T>(raw[u], val);
         const int c0 = row.first_column(v);
-        if (usual) {
-            const Pair scale = pair(s.s2, s.s2), a = pair(-r2, -r2), b = pair(-l2, -l2), k1 = pair(slope, slope), k0 = pair(level, level);
+        const Pair scale = pair(s.s2, s.s2), a = pair(-state.x, -state.x), b = pair(-state.y, -state.y), k1 = pair(slope, slope), k0 = pair(level, level);
 #pragma unroll
-            for (int j = 0; j < V; j += 2) {
-                float2 d = halves(add_pair(fma_pair(pair(val[j], val[j + 1]), scale, a), b));
-                d.x = max_or_nan(d.x, kFarBelow), d.y = max_or_nan(d.y, kFarBelow);
-                const float2 got = halves(mul_pair(pair(ex2(d.x), ex2(d.y)), fma_pair(k1, pair(d.x, d.y), k0)));
-                val[j] = val[j] == -INFINITY ? 0.f : got.x;
-                val[j + 1] = val[j + 1] == -INFINITY ? 0.f : got.y;
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < V; ++j) val[j] = gradient(val[j]);
+        for (int j = 0; j < V; j += 2) {
+            float2 d = halves(fma_pair(add_pair(pair(val[j], val[j + 1]), a), scale, b));
+            d.x = max_or_nan(d.x, kFarBelow), d.y = max_or_nan(d.y, kFarBelow);
+            const float2 got = halves(mul_pair(pair(ex2(d.x), ex2(d.y)), fma_pair(k1, pair(d.x, d.y), k0)));
+            val[j] = val[j] == -INFINITY ? 0.f : got.x;
+            val[j + 1] = val[j + 1] == -INFINITY ? 0.f : got.y;
         }
         const unsigned at = (unsigned)(target - c0);
         if (at < (unsigned)V && target >= 0 && g_target != 0.f) {

@@ -8,7 +8,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 import device_op_forms as forms  # noqa: E402
-from test_device_ops_gpu import TYPES, check_log_probs, cuda, gen, ops  # noqa: E402, F401
+from test_device_ops_gpu import TYPES, check_log_probs, cuda, gen, grad_tolerance, log_tolerance, ops  # noqa: E402, F401
 
 pytestmark = pytest.mark.gpu
 
@@ -72,3 +72,39 @@ def test_a_live_nan_among_hidden_columns(ops, size, hidden, dtype):  # noqa: F81
     assert torch.equal(torch.isnan(got.log_sum).cpu(), lost)
     grad = ops.log_probs_grad(x.cuda(), got, grad_log_prob=torch.ones(rows).cuda()).cpu()
     assert torch.equal(torch.isnan(grad), live & lost[:, None]) and torch.all(grad[~live] == 0)
+
+
+@pytest.mark.parametrize("far", [-1e9, -3e9, -1e10, -1e20, 1e10, 1e20])
+@pytest.mark.parametrize("dtype,scale", [(torch.float32, 1.0), (torch.bfloat16, 0.5), (torch.float16, 1e6)])
+@pytest.mark.parametrize("cols", [5000, 70_001])
+def test_scores_far_from_the_others(ops, cols, dtype, scale, far):  # noqa: F811
+    """Finite numbers that stand for hidden columns, or for the one answer: logits whose rounding in fp32 is more than a power of two's
+    whole range.  A row's own differences are what counts; equal scores share the row however far out they are."""
+    far = max(-65504.0, min(65504.0, far / scale)) if dtype == torch.float16 else far
+    g = gen(cols)
+    x = (torch.randn(8, cols, generator=g) * (3 / max(scale, 1.0))).to(dtype)
+    x[0] = far
+    x[1, : cols // 2] = far
+    x[2, -40:] = far
+    x[3, : cols - cols // 10] = far
+    x[4] = far
+    x[4, cols - 1] = 1.0
+    x[5].view(-1, 8 if cols % 8 == 0 else 1)[::2] = far
+    x[6] = far
+    x[6, ::3] = -math.inf
+    x[7, 4] = far
+    target = torch.tensor([3, 5, cols - 1, cols - 2, cols - 1, 2, 1, 4], dtype=torch.int32)
+    weights = [torch.randn(shape, generator=g) / max(scale, 1.0) for shape in ((8,), (8,), (8, 5))]
+    want = forms.log_probs(x, target, scale=scale, n_best=5)
+    got = ops.log_probs(x.cuda(), target.cuda(), scale=scale, n_best=5)
+    for name in ("log_prob", "log_sum", "best_log_prob"):
+        a, b = getattr(got, name).cpu().double(), want[name]
+        assert torch.all((a - b).abs() <= log_tolerance(cols, b)), (name, a, b)
+    a, b = got.entropy.cpu().double(), want["entropy"]
+    assert torch.all((a - b).abs() <= log_tolerance(cols, b) * (1 + b))
+    assert torch.equal(got.best_index.cpu(), want["best_index"])
+    grad = ops.log_probs_grad(x.cuda(), got, grad_log_prob=weights[0].cuda(), grad_entropy=weights[1].cuda(), grad_best=weights[2].cuda()).cpu().double()
+    right = forms.log_probs_grad(x, want, target, scale, *weights)
+    total = weights[0].double().abs() + weights[2].double().abs().sum(1)
+    tol = grad_tolerance(want, dtype, total, weights[1].double(), scale, cols, right)
+    assert torch.all((grad - right).abs() <= tol), ((grad - right).abs() / tol).max()
