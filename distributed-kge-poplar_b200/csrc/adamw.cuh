@@ -98,7 +98,7 @@ constexpr int kBlocksPerWarp = 2;  // fetched together
 
 __device__ __forceinline__ float quick_sqrt(float x) {
     float y;
-    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 __device__ __forceinline__ float quick_reciprocal(float x) {
@@ -179,7 +179,9 @@ struct Step {
           step_size(a.step_size), correction(a.correction), key(a.key) {
         if (a.schedule) decay = a.schedule[0], step_size = a.schedule[1], correction = a.schedule[2], key = __float_as_uint(a.schedule[3]);
     }
-    // Root and reciprocal to 2^-22: the step that they scale is a thousandth of the parameter, whose own rounding is 2^-24 or more.
+    // Root and reciprocal to 2^-22: the step that they scale is a thousandth of the parameter, whose own rounding is 2^-24 or more.  The
+    // root's bound holds for every v, subnormal ones included (gradients below 3e-18 make such; taken for 0 they left epsilon alone to
+    // divide by), the reciprocal's from 2^-126 to 2^126: epsilon is a normal number, and a root is below 2^64.
     __device__ __forceinline__ void take(float& p, float g, float& m, float& v) const {
         m = fmaf(beta_m, m, one_minus_beta_m * g);
         v = fmaf(beta_v, v, one_minus_beta_v * g * g);

@@ -4,6 +4,7 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <type_traits>
 
@@ -368,6 +369,8 @@ void adamw_step(const kge_adamw_args& a, const kge_adamw_tensor* tensors, size_t
     if (a.param_type != KGE_F32 && a.param_type != KGE_BF16) fail(KGE_INVALID_ARGUMENT, msg() << what << ": parameters must be KGE_F32 or KGE_BF16, not " << a.param_type);
     const size_t param_bytes = a.param_type == KGE_F32 ? 4 : 2, grad_bytes = type_bytes(a.grad_type, what);
     if (a.state_bits != 8 && a.state_bits != 32) fail(KGE_INVALID_ARGUMENT, msg() << what << ": state_bits must be 8 or 32, not " << a.state_bits);
+    // (float)epsilon must be a normal number: 0 makes 0 / 0 of values that have had no gradient yet
+    if (!((float)a.epsilon >= FLT_MIN && (float)a.epsilon <= FLT_MAX)) fail(KGE_INVALID_ARGUMENT, msg() << what << ": epsilon must be a normal fp32 number above 0, not " << a.epsilon);
     need(n_tensors == 0 || tensors, "kge_op_adamw: null tensors");
     const adamw::Params p{(float)a.beta_m, (float)((1. - a.beta_m) * a.grad_scale), (float)a.beta_v, (float)((1. - a.beta_v) * a.grad_scale * a.grad_scale), (float)a.epsilon,
                           (float)a.decay, (float)a.step_size, (float)a.inv_sqrt_correction, a.key, a.schedule};

@@ -124,8 +124,8 @@ class AdamW:
             raise ValueError(f"state_bits must be 8 or 32, not {state_bits}")
         if not (0 <= beta_m < 1 and 0 <= beta_v < 1):
             raise ValueError(f"beta_m and beta_v must be at least 0 and below 1, not {beta_m} and {beta_v}")
-        if not epsilon > 0:
-            raise ValueError(f"epsilon must be positive, not {epsilon}")
+        if not torch.finfo(torch.float32).tiny <= epsilon <= torch.finfo(torch.float32).max:
+            raise ValueError(f"epsilon must be positive and a normal number in float32, not {epsilon}")
         for i, p in enumerate(self.params):
             _must_be_tensor(f"parameter {i}", p)
         self._tensors = _module.AdamWTensors(self.params)

@@ -8,7 +8,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 import device_op_forms as forms  # noqa: E402
-from test_device_ops_gpu import TYPES, check_log_probs, cuda, gen, grad_tolerance, log_tolerance, ops  # noqa: E402, F401
+from test_device_ops_gpu import TYPES, U, check_log_probs, cuda, gen, grad_tolerance, log_tolerance, ops  # noqa: E402, F401
 
 pytestmark = pytest.mark.gpu
 
@@ -108,3 +108,17 @@ def test_scores_far_from_the_others(ops, cols, dtype, scale, far):  # noqa: F811
     total = weights[0].double().abs() + weights[2].double().abs().sum(1)
     tol = grad_tolerance(want, dtype, total, weights[1].double(), scale, cols, right)
     assert torch.all((grad - right).abs() <= tol), ((grad - right).abs() / tol).max()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_of_tiny_gradients(ops, bits):  # noqa: F811
+    """Second moments that are subnormal in fp32 count: (1 - beta_v) g^2 and its sum are off by a step of subnormal numbers, 2^-149, which
+    moves the root by that over 2 v of itself.  A step in 8 bits divides by the sum before it is encoded."""
+    g = torch.exp(torch.linspace(math.log(2e-20), math.log(3e-16), 4096).double()).float() * torch.tensor([1.0, -1.0]).repeat(2048)
+    p = torch.zeros(4096).cuda()
+    optimiser = ops.AdamW([p], state_bits=bits, beta_m=0.9, beta_v=0.999, epsilon=1e-20)
+    optimiser.step([g.cuda()], 0.01)
+    m, v = 0.1 * g.double(), 0.001 * g.double() ** 2
+    want = -0.01 * (m / 0.1) / ((v / 0.001).sqrt() + 1e-20)
+    off = 2.0**-149 / (2 * v) + 32 * U
+    assert torch.all((p.cpu().double() - want).abs() <= off * want.abs())
