@@ -179,13 +179,17 @@ struct Step {
           step_size(a.step_size), correction(a.correction), key(a.key) {
         if (a.schedule) decay = a.schedule[0], step_size = a.schedule[1], correction = a.schedule[2], key = __float_as_uint(a.schedule[3]);
     }
-    // Root and reciprocal to 2^-22: the step that they scale is a thousandth of the parameter, whose own rounding is 2^-24 or more.  The
-    // root's bound holds for every v, subnormal ones included (gradients below 3e-18 make such; taken for 0 they left epsilon alone to
-    // divide by), the reciprocal's from 2^-126 to 2^126: epsilon is a normal number, and a root is below 2^64.
+    // With 32-bit moments root and division are rounded to nearest, in the shade of the bytes (60 M values 228 us, with the approximations
+    // below 231).  With 8-bit ones, whose step is bound by instructions, they are right to 2^-22 (120 M values 444 us, to nearest 500): the
+    // step that they scale is a thousandth of the parameter, whose own rounding is 2^-24 or more.  The root's bound holds for every v, subnormal
+    // ones included (gradients below 3e-18 make such; taken for 0 they left epsilon alone to divide by), the reciprocal's from 2^-126 to
+    // 2^126: epsilon is a normal number, and a root is below 2^64.
+    template <bool NEAREST>
     __device__ __forceinline__ void take(float& p, float g, float& m, float& v) const {
         m = fmaf(beta_m, m, one_minus_beta_m * g);
         v = fmaf(beta_v, v, one_minus_beta_v * g * g);
-        p = fmaf(p, decay, -step_size * m * quick_reciprocal(fmaf(quick_sqrt(v), correction, epsilon)));
+        if (NEAREST) p = fmaf(p, decay, __fdiv_rn(-step_size * m, fmaf(__fsqrt_rn(v), correction, epsilon)));
+        else p = fmaf(p, decay, -step_size * m * quick_reciprocal(fmaf(quick_sqrt(v), correction, epsilon)));
     }
     // What is mixed for the values from a position (a multiple of 4) on.
     __device__ __forceinline__ uint32_t mixed(unsigned long long at) const { return (uint32_t)at * 0x9E3779B9u + (uint32_t)(at >> 32) * 0x6A09E667u + key; }
@@ -266,7 +270,7 @@ static __global__ void __launch_bounds__(kThreads, 3) k_adamw32(const __grid_con
         g_raw[u].floats(g);
         // past the tensor's end gradient and moments are 0, and stay so
 #pragma unroll
-        for (int j = 0; j < 4; ++j) step.take(p[j], g[j], m[j], v[j]);
+        for (int j = 0; j < 4; ++j) step.take<true>(p[j], g[j], m[j], v[j]);
         uint32_t draw[4] = {};
         if constexpr (sizeof(TP) == 2) {
 #pragma unroll
@@ -382,7 +386,7 @@ static __global__ void __launch_bounds__(kThreads, 3) k_adamw8(const __grid_cons
         // past the tensor's end gradient and moments are 0, and stay so
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            step.take(p[j], g[j], m[4 * q + j], v[4 * q + j]);
+            step.take<false>(p[j], g[j], m[4 * q + j], v[4 * q + j]);
             d[j] = draw[4 * q + j] = mix(base + (uint32_t)(4 * q + j) * 0x9E3779B9u);
             largest_m = max_or_nan(largest_m, fabsf(m[4 * q + j]));
             largest_v = max_or_nan(largest_v, v[4 * q + j]);

@@ -3,6 +3,7 @@ that are thinned out, larger blocks, tiles and parts."""
 
 import math
 
+import numpy as np
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -122,3 +123,21 @@ def test_adamw_of_tiny_gradients(ops, bits):  # noqa: F811
     want = -0.01 * (m / 0.1) / ((v / 0.001).sqrt() + 1e-20)
     off = 2.0**-149 / (2 * v) + 32 * U
     assert torch.all((p.cpu().double() - want).abs() <= off * want.abs())
+
+
+def test_a_step_of_32_bits_is_rounded_as_its_formula_is(ops):  # noqa: F811
+    """The first step in numpy's fp32 arithmetic, its two fused operations in 64 bits and rounded once more: that differs from a fused one
+    only where 53 bits end in a half of 24, once in 2^28."""
+    n = 1 << 16
+    g = (torch.randn(n, generator=gen(5)) * torch.exp(2 * torch.randn(n, generator=gen(6)))).numpy()
+    p0 = torch.randn(n, generator=gen(7)).numpy()
+    p = torch.from_numpy(p0).cuda()
+    optimiser = ops.AdamW([p], beta_m=0.9, beta_v=0.999, epsilon=1e-8, weight_decay=0.1)
+    optimiser.step([torch.from_numpy(g).cuda()], 0.01)
+    f = np.float32
+    m, v = f(1 - 0.9) * g, f(1 - 0.999) * g * g
+    assert np.array_equal(optimiser.adam_m[:n].cpu().numpy(), m) and np.array_equal(optimiser.adam_v[:n].cpu().numpy(), v)
+    under = (np.sqrt(v).astype(np.float64) * f((1 - 0.999) ** -0.5) + np.float64(f(1e-8))).astype(f)
+    step = -f(0.01 / (1 - 0.9)) * m / under
+    want = (p0.astype(np.float64) * f(1 - 0.01 * 0.1) + step).astype(f)
+    assert np.array_equal(p.cpu().numpy(), want)
