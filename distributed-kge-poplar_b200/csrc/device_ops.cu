@@ -371,6 +371,13 @@ void adamw_step(const kge_adamw_args& a, const kge_adamw_tensor* tensors, size_t
     if (a.state_bits != 8 && a.state_bits != 32) fail(KGE_INVALID_ARGUMENT, msg() << what << ": state_bits must be 8 or 32, not " << a.state_bits);
     // (float)epsilon must be a normal number: 0 makes 0 / 0 of values that have had no gradient yet
     if (!((float)a.epsilon >= FLT_MIN && (float)a.epsilon <= FLT_MAX)) fail(KGE_INVALID_ARGUMENT, msg() << what << ": epsilon must be a normal fp32 number above 0, not " << a.epsilon);
+    // (1 - beta) times the scale, or its square, is one fp32 factor: where that is no normal number the moments would be lost or infinite
+    const auto held = [&](double beta, double scale) {
+        const float factor = (float)std::fabs((1. - beta) * scale);
+        return beta == 1. || scale == 0. || !std::isfinite(a.grad_scale) || (factor >= FLT_MIN && factor <= FLT_MAX);
+    };
+    if (!held(a.beta_m, a.grad_scale) || !held(a.beta_v, a.grad_scale * a.grad_scale) || (a.grad_scale != 0. && a.grad_scale * a.grad_scale == 0.))
+        fail(KGE_INVALID_ARGUMENT, msg() << what << ": grad_scale is " << a.grad_scale << ": (1 - beta) times its square must be a normal fp32 number");
     need(n_tensors == 0 || tensors, "kge_op_adamw: null tensors");
     const adamw::Params p{(float)a.beta_m, (float)((1. - a.beta_m) * a.grad_scale), (float)a.beta_v, (float)((1. - a.beta_v) * a.grad_scale * a.grad_scale), (float)a.epsilon,
                           (float)a.decay, (float)a.step_size, (float)a.inv_sqrt_correction, a.key, a.schedule};

@@ -161,8 +161,9 @@ class AdamW:
     def step(self, grads: Sequence[Optional[torch.Tensor]], learning_rate: Optional[float] = None, *,
              schedule: Optional[torch.Tensor] = None, grad_scale: float = 1.0) -> None:
         """One step with ``grads`` (one per parameter, all of one type, contiguous; None: the parameter and its moments stay as they
-        are), each multiplied by ``grad_scale``.  Either ``learning_rate`` is given and the step is counted, or ``schedule``, which
-        :meth:`advance` has written.  A step under stream capture needs a schedule: its replays would repeat one step's number."""
+        are), each multiplied by ``grad_scale`` (from about 1e-17 to 1e20, since its square goes into the second moments; or 0).  Either
+        ``learning_rate`` is given and the step is counted, or ``schedule``, which :meth:`advance` has written.  A step under stream
+        capture needs a schedule: its replays would repeat one step's number."""
         if (learning_rate is None) == (schedule is None):
             raise ValueError("step() takes a learning_rate or a schedule")
         if schedule is not None:

@@ -386,7 +386,8 @@ typedef struct kge_adamw_args {
     int state_bits;       /* 8 or 32 */
     void *adam_m, *adam_v;            /* fp32 or bytes; aligned to 16 bytes */
     uint8_t *m_exponent, *v_exponent; /* 8 bits only */
-    double beta_m, beta_v, epsilon, grad_scale; /* 1 - beta is taken before anything is rounded to fp32; epsilon is a normal fp32 number */
+    double beta_m, beta_v, epsilon, grad_scale; /* 1 - beta is taken before anything is rounded to fp32; epsilon, and 1 - beta times
+                                                   grad_scale or its square (unless 0), are normal fp32 numbers */
     double decay, step_size, inv_sqrt_correction;
     uint32_t key;
     const float* schedule; /* not NULL: decay, step_size, inv_sqrt_correction and the key's bits are read from these four words on

@@ -13,3 +13,8 @@ def test_an_epsilon_that_is_no_normal_number_in_fp32(epsilon):
     refused(adamw(epsilon=epsilon), "epsilon")
     with pytest.raises(ValueError, match="epsilon"):
         device_ops.AdamW([torch.zeros(3)], epsilon=epsilon)
+
+
+@pytest.mark.parametrize("scale", [1e-20, -1e-20, 1e-200, 1e25, -1e25, 1e160])
+def test_a_gradient_scale_whose_square_fp32_does_not_hold(scale):
+    refused(adamw(grad_scale=scale), "grad_scale")
