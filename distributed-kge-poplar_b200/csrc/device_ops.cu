@@ -330,6 +330,7 @@ void product8(const uint8_t* a_values, const uint8_t* a_exponents, size_t m, con
 
 bool product8_gave_up() {
     unsigned status = 0;
+    KGE_CUDA(cudaDeviceSynchronize());  // the copy alone would not wait for streams that do not wait for the default stream
     KGE_CUDA(cudaMemcpyFromSymbol(&status, rows8::g_product8_status, sizeof status));
     if (status) {
         const unsigned zero = 0;

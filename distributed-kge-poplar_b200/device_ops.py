@@ -2,6 +2,7 @@
 
   log_probs, log_probs_grad   log probability of a given candidate per row of scores, entropy and the n_best alternatives
   quantise_rows, product8     scores as a product of rows in 8-bit floating point with a power of two for each 128 values
+  check_product8              whether the product's bounded waits have all ended well
   AdamW                       one step over many tensors, moments in 32 or in 8 bits
 
 They are the ``kge_op_*`` entry points for device arrays of ``include/kge_b200.h``, which states their arithmetic, with torch
@@ -16,6 +17,7 @@ parameter after another (src/fructose/frnn.cpp:61-90).
 
 from __future__ import annotations
 
+import contextlib
 import importlib.util
 from pathlib import Path
 from typing import Any, Dict, Optional, Sequence, Tuple, Union
@@ -100,10 +102,21 @@ def product8(a: Union[torch.Tensor, Rows8], b: Union[torch.Tensor, Rows8], *, dt
     """``out[i, j] = sum_c a[i, c] * b[j, c]`` [a.rows, b.rows] of rows in 8-bit floating point, summed in 32 bits; a tensor is
     quantised by the call.  Scores of queries ``a`` against a table ``b``; their gradients are the products
     ``product8(grad, quantise_rows(b, transposed=True))`` and
-    ``product8(quantise_rows(grad, transposed=True), quantise_rows(a, transposed=True))``."""
+    ``product8(quantise_rows(grad, transposed=True), quantise_rows(a, transposed=True))``.  :func:`check_product8` tells whether the
+    device has kept to it."""
     a = a if isinstance(a, Rows8) else quantise_rows(a)
     b = b if isinstance(b, Rows8) else quantise_rows(b)
     return _module.product8(a, b, dtype, out)
+
+
+def check_product8(device: Union[torch.device, int, None] = None) -> None:
+    """Waits for the device (None: the current one) and raises ``RuntimeError`` if a wait inside a :func:`product8` on it has given up
+    since the last question: the product's waits are bounded, and one that ran out leaves results that are not to be used."""
+    lib = capi.load_library()
+    with contextlib.nullcontext() if device is None else torch.cuda.device(device):
+        status = lib.kge_op_product8_status()
+    if status != capi.OK:
+        raise RuntimeError(lib.kge_last_error(None).decode())
 
 
 class AdamW:

@@ -4,7 +4,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from distributed_kge_poplar_b200 import device_ops  # noqa: E402
+from distributed_kge_poplar_b200 import capi, device_ops  # noqa: E402
 from test_device_ops_cpu import adamw, refused  # noqa: E402
 
 
@@ -18,3 +18,20 @@ def test_an_epsilon_that_is_no_normal_number_in_fp32(epsilon):
 @pytest.mark.parametrize("scale", [1e-20, -1e-20, 1e-200, 1e25, -1e25, 1e160])
 def test_a_gradient_scale_whose_square_fp32_does_not_hold(scale):
     refused(adamw(grad_scale=scale), "grad_scale")
+
+
+def test_a_product_that_gave_up_is_an_error(monkeypatch):
+    class Library:  # answers as the library does after a wait on the device has run out
+        status = capi.DEVICE_STATUS
+
+        def kge_op_product8_status(self):
+            return self.status
+
+        def kge_last_error(self, engine):
+            return b"kge_op_product8: a wait on the device gave up"
+
+    monkeypatch.setattr(capi, "load_library", Library)
+    with pytest.raises(RuntimeError, match="a wait on the device gave up"):
+        device_ops.check_product8()
+    monkeypatch.setattr(Library, "status", capi.OK)
+    device_ops.check_product8()

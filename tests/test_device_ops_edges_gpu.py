@@ -141,3 +141,16 @@ def test_a_step_of_32_bits_is_rounded_as_its_formula_is(ops):  # noqa: F811
     step = -f(0.01 / (1 - 0.9)) * m / under
     want = (p0.astype(np.float64) * f(1 - 0.01 * 0.1) + step).astype(f)
     assert np.array_equal(p.cpu().numpy(), want)
+
+
+def test_the_product_s_status_waits_for_every_stream(ops):  # noqa: F811
+    x = torch.randn(200, 300).cuda()
+    ops.product8(x, x)  # the first call of a kernel loads it and waits
+    ops.check_product8()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)  # a tenth of a second
+        ops.product8(x, x)
+    ops.check_product8()
+    assert side.query()
