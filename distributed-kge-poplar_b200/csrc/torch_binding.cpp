@@ -73,6 +73,16 @@ std::pair<uintptr_t, uintptr_t> span(const Tensor& t) {
     for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
     return {first, first + (uintptr_t)(last + 1) * t.element_size()};
 }
+// What is written must not be what is read beside it.  `b` undefined or either empty: nothing to say.
+void must_not_overlap(const char* what_a, const Tensor& a, const char* what_b, const Tensor& b) {
+    if (!b.defined() || a.numel() == 0 || b.numel() == 0) return;
+    const auto [a_first, a_end] = span(a);
+    const auto [b_first, b_end] = span(b);
+    if (a_first < b_end && b_first < a_end) refuse(what_a, " and ", what_b, " overlap in memory");
+}
+void must_not_overlap(const char* what_a, const Tensor& a, const char* what_b, const OptionalTensor& b) {
+    if (b) must_not_overlap(what_a, a, what_b, *b);
+}
 void* stream_of(c10::Device device) { return c10::cuda::getCurrentCUDAStream(device.index()).stream(); }
 
 // ---------------------------------------------------------------------------
@@ -169,11 +179,14 @@ Tensor log_probs_grad(const Tensor& scores, const LogProbs& r, const OptionalTen
         must_be_with("out", out, scores.device());
         must_have_shape("out", out, scores.sizes());
         must_be_matrix("out", out);
-        if (out.numel() && (out.data_ptr() != scores.data_ptr() || rows_apart(out) != rows_apart(scores))) {
-            const auto [first, end] = span(out);
-            const auto [scores_first, scores_end] = span(scores);
-            if (first < scores_end && scores_first < end) refuse("out and scores overlap in memory");
-        }
+        if (out.data_ptr() != scores.data_ptr() || rows_apart(out) != rows_apart(scores)) must_not_overlap("out", out, "scores", scores);
+        must_not_overlap("out", out, "the result", r.memory);
+        must_not_overlap("out", out, "target", r.target);
+        must_not_overlap("out", out, "mask", r.mask);
+        must_not_overlap("out", out, "count", r.count);
+        must_not_overlap("out", out, "grad_log_prob", a);
+        must_not_overlap("out", out, "grad_entropy", b);
+        must_not_overlap("out", out, "grad_best", c);
         out.unsafeGetTensorImpl()->bump_version();
     } else {
         out = at::empty(scores.sizes(), scores.options());
@@ -218,6 +231,10 @@ Tensor product8(const Rows8& a, const Rows8& b, at::ScalarType dtype, const Opti
         must_be_with("out", out, device);
         must_have_shape("out", out, {a.rows, b.rows});
         must_be_matrix("out", out);
+        must_not_overlap("out", out, "a", a.values);
+        must_not_overlap("out", out, "a", a.exponents);
+        must_not_overlap("out", out, "b", b.values);
+        must_not_overlap("out", out, "b", b.exponents);
         out.unsafeGetTensorImpl()->bump_version();
     } else {
         must_be_float("dtype", dtype);
@@ -239,6 +256,7 @@ struct AdamWTensors {
     std::vector<Tensor> params;
     std::vector<kge_adamw_tensor> table;
     std::vector<int64_t> first, sizes;
+    std::vector<size_t> order;  // of those that are not empty, by where they lay
     at::ScalarType type;
     int64_t total = 0;
 
@@ -265,6 +283,29 @@ struct AdamWTensors {
             total += (p.numel() + 127) / 128 * 128;
         }
         std::sort(spans.begin(), spans.end());
+        refuse_neighbours(spans);
+        for (const auto& s : spans) order.push_back(std::get<2>(s));
+    }
+
+    // The parameters of a step may not overlap one another (their memory may have been replaced) nor its gradients.  They are gone through
+    // in the order that they lay in at first; one that has moved costs a sort.
+    void must_not_meet(size_t grad_bytes) const {
+        std::vector<std::tuple<uintptr_t, uintptr_t, size_t>> spans;
+        for (const size_t i : order)
+            if (table[i].size) {
+                const auto first = reinterpret_cast<uintptr_t>(table[i].param);
+                spans.emplace_back(first, first + table[i].size * params[i].element_size(), i);
+            }
+        if (!std::is_sorted(spans.begin(), spans.end())) std::sort(spans.begin(), spans.end());
+        refuse_neighbours(spans);
+        for (size_t i = 0; i < table.size(); ++i) {
+            if (!table[i].size) continue;
+            const auto first = reinterpret_cast<uintptr_t>(table[i].grad), end = first + table[i].size * grad_bytes;
+            const auto next = std::lower_bound(spans.begin(), spans.end(), end, [](const auto& s, uintptr_t at) { return std::get<0>(s) < at; });
+            if (next != spans.begin() && std::get<1>(*std::prev(next)) > first) refuse("gradient ", i, " and parameter ", std::get<2>(*std::prev(next)), " overlap in memory");
+        }
+    }
+    static void refuse_neighbours(const std::vector<std::tuple<uintptr_t, uintptr_t, size_t>>& spans) {
         for (size_t i = 1; i < spans.size(); ++i)
             if (std::get<0>(spans[i]) < std::get<1>(spans[i - 1])) refuse("parameters ", std::get<2>(spans[i - 1]), " and ", std::get<2>(spans[i]), " overlap in memory");
     }
@@ -323,6 +364,7 @@ struct AdamWTensors {
             if (!schedule->is_contiguous()) refuse("schedule must be contiguous");
             a.schedule = schedule->data_ptr<float>();
         }
+        must_not_meet(c10::elementSize(*grad_type));
         const c10::cuda::CUDAGuard guard(device);
         check(kge_op_adamw(&a, table.data(), table.size(), stream_of(device)));
         for (size_t i = 0; i < params.size(); ++i)

@@ -277,6 +277,7 @@ int kge_op_all_to_all(const float* in, size_t n_shard, size_t block, float* out)
  *     long as they share no output and no workspace.
  *   - `workspace` is `workspace_bytes` of device memory, aligned to 256 bytes, whose contents need not be anything before the
  *     call and are nothing after it; how much is wanted is asked of the ..._workspace function (0: NULL will do).
+ *   - what a call writes may not overlap what it reads, but where it says so.
  *   - float_type is KGE_F32, KGE_F16 or KGE_BF16; arithmetic is in 32 bits, results are rounded once.
  *   - sizes of zero are no error: nothing is launched that has nothing to write.
  */

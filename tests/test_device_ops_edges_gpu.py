@@ -154,3 +154,44 @@ def test_the_product_s_status_waits_for_every_stream(ops):  # noqa: F811
         ops.product8(x, x)
     ops.check_product8()
     assert side.query()
+
+
+def test_outputs_that_overlap_what_is_read_are_refused(ops):  # noqa: F811
+    x = torch.randn(6, 8).cuda()
+    r = ops.log_probs(x, torch.zeros(6, dtype=torch.int32).cuda(), n_best=8)
+    ones = torch.ones(6, 8).cuda()
+    a, b = ops.quantise_rows(torch.randn(64, 128).cuda()), ops.quantise_rows(torch.randn(16, 128).cuda())
+    for call, text in [(lambda: ops.log_probs_grad(x, r, out=r.best_log_prob), "out and the result"),
+                       (lambda: ops.log_probs_grad(x, r, grad_best=ones, out=ones), "out and grad_best"),
+                       (lambda: ops.log_probs_grad(x, r, grad_log_prob=ones.view(-1)[:6], out=ones), "out and grad_log_prob"),
+                       (lambda: ops.log_probs_grad(x, ops.log_probs(x, ones.view(torch.int32)[0, :6]), out=ones), "out and target"),
+                       (lambda: ops.log_probs_grad(x, ops.log_probs(x, count=ones.view(torch.int32)[0, :6]), out=ones), "out and count"),
+                       (lambda: ops.log_probs_grad(x, ops.log_probs(x, mask=ones.view(torch.uint8)[:6, 4:12]), out=ones), "out and mask"),
+                       (lambda: ops.product8(a, b, out=a.values.view(torch.bfloat16).view(-1)[: 64 * 16].view(64, 16)), "out and a overlap"),
+                       (lambda: ops.product8(b, a, out=a.values.view(torch.bfloat16).view(-1)[: 64 * 16].view(16, 64)), "out and b overlap"),
+                       (lambda: ops.product8(b, b, out=a.exponents.view(torch.bfloat16).view(16, 16)), None)]:
+        if text is None:
+            call()
+            continue
+        with pytest.raises(ValueError, match=text):
+            call()
+    assert torch.equal(ops.log_probs_grad(x.clone(), r, grad_best=ones), ops.log_probs_grad(x, r, grad_best=ones, out=x))  # in place is no overlap
+
+
+def test_parameters_that_overlap_a_gradient_or_one_another_are_refused(ops):  # noqa: F811
+    base = torch.zeros(400).cuda()
+    params = [base[200:300], base[:100], torch.zeros(0).cuda(), torch.zeros(50).cuda()]
+    optimiser = ops.AdamW(params)
+    apart = [torch.ones(100).cuda(), torch.ones(100).cuda(), torch.zeros(0).cuda(), torch.ones(50).cuda()]
+    for i, grad, text in [(0, base[200:300], "gradient 0 and parameter 0"), (0, base[1:101], "gradient 0 and parameter 1"),
+                          (1, base[299:399], "gradient 1 and parameter 0"), (3, base[170:220], "gradient 3 and parameter 0")]:
+        with pytest.raises(ValueError, match=text + " overlap"):
+            optimiser.step([grad if j == i else g for j, g in enumerate(apart)], 0.1)
+    params[3].data = base[80:130]
+    with pytest.raises(ValueError, match="parameters 1 and 3 overlap"):
+        optimiser.step(apart, 0.1)
+    assert optimiser.step_count == 0 and torch.all(base == 0)
+    optimiser.step([base[300:400], base[100:200], None, None], 0.1)  # side by side
+    params[3].data = base[130:180]
+    optimiser.step([torch.ones(100).cuda()] * 2 + [None, torch.ones(50).cuda()], 0.1)  # moved, and one gradient for two
+    assert torch.all(base[130:180] < 0) and torch.all(base[180:200] == 0)
