@@ -161,14 +161,18 @@ class AdamW:
         return torch.zeros(4, dtype=torch.float32, device=self.device)
 
     def advance(self, schedule: torch.Tensor, learning_rate: float) -> None:
-        """Counts a step and writes what it needs into ``schedule``: before each replay of a graph that holds
-        ``step(grads, schedule=schedule)``."""
+        """Counts a step and writes what it needs into ``schedule``, on the current stream: before each replay of a graph that holds
+        ``step(grads, schedule=schedule)``.  The host does not wait: steps may be queued ahead."""
         if schedule.shape != (4,) or schedule.dtype != torch.float32:
             raise ValueError("schedule must be what new_schedule() gave")
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("advance() is called before a graph's replay, not under its capture")
         decay, step_size, correction, key = self._scalars(learning_rate, self.step_count + 1)
-        words = torch.tensor([decay, step_size, correction, 0.0], dtype=torch.float32)
+        # page-locked: of other memory the copy would wait for the stream; torch lends it anew once the copy is done
+        words = torch.empty(4, dtype=torch.float32, pin_memory=True)
+        words.copy_(torch.tensor([decay, step_size, correction, 0.0], dtype=torch.float32))
         words.view(torch.int32)[3] = key - (1 << 32) if key >> 31 else key
-        schedule.copy_(words)
+        schedule.copy_(words, non_blocking=True)
         self.step_count += 1
 
     def step(self, grads: Sequence[Optional[torch.Tensor]], learning_rate: Optional[float] = None, *,

@@ -195,3 +195,31 @@ def test_parameters_that_overlap_a_gradient_or_one_another_are_refused(ops):  # 
     params[3].data = base[130:180]
     optimiser.step([torch.ones(100).cuda()] * 2 + [None, torch.ones(50).cuda()], 0.1)  # moved, and one gradient for two
     assert torch.all(base[130:180] < 0) and torch.all(base[180:200] == 0)
+
+
+def test_a_schedule_is_written_without_waiting(ops):  # noqa: F811
+    """Replays are queued behind a stream that is busy; each reads its own step's words all the same."""
+    g = gen(4)
+    start, grad = torch.randn(1000, generator=g), torch.randn(1000, generator=g).cuda()
+    p, q = start.cuda(), start.cuda()
+    one, other = ops.AdamW([p], state_bits=8, seed=3), ops.AdamW([q], state_bits=8, seed=3)
+    one.step([grad], 0.01)
+    schedule = other.new_schedule()
+    other.advance(schedule, 0.01)
+    other.step([grad], schedule=schedule)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        other.step([grad], schedule=schedule)
+    torch.cuda.synchronize()
+    torch.cuda._sleep(400_000_000)  # a fifth of a second
+    for i in range(20):
+        other.advance(schedule, 0.01 / (i + 1))
+        graph.replay()
+    assert not torch.cuda.current_stream().query()
+    for i in range(20):
+        one.step([grad], 0.01 / (i + 1))
+    assert torch.equal(p, q) and torch.equal(one.adam_m, other.adam_m) and torch.equal(one.adam_v, other.adam_v)
+    with pytest.raises(RuntimeError, match="not under its capture"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            other.advance(schedule, 0.01)
+    assert other.step_count == 21
