@@ -6,12 +6,13 @@ Produces, next to this file:
   libkge_b200.so              the C ABI of include/kge_b200.h (CUDA runtime only)
   libpoplar_kge<ext-suffix>   the pybind11 module with the reference's `Engine` class
   libkge_torch<ext-suffix>    the operators on device arrays for torch tensors (the only part that knows torch)
-A target is rebuilt when any source or header is newer than it.
+A target is rebuilt when any source or header is newer than it, the last one also when torch is another version.
 """
 
 from __future__ import annotations
 
 import argparse
+import importlib.metadata
 import os
 import shutil
 import subprocess
@@ -19,6 +20,7 @@ import sys
 import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
+from typing import Optional
 
 HERE = Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
@@ -74,20 +76,42 @@ def build(force: bool = False, verbose: bool = False) -> None:
             ],
             verbose,
         )
-    binding = CSRC / "torch_binding.cpp"
-    if force or _newer_than(TORCH_MODULE, [binding, INCLUDE / "kge_b200.h"]):
-        from torch.utils import cpp_extension
+    _build_torch_module(force, verbose)
 
-        includes = [f"-I{p}" for p in cpp_extension.include_paths("cuda") + [sysconfig.get_paths()["include"], INCLUDE]]
-        torch_libs = [f"-L{p}" for p in cpp_extension.library_paths()]
-        _run(
-            [
-                os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-Wall", "-DTORCH_EXTENSION_NAME=libkge_torch", *includes,
-                binding, "-o", TORCH_MODULE, f"-L{HERE}", "-lkge_b200", *torch_libs, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10",
-                "-lc10_cuda", "-Wl,-rpath,$ORIGIN",
-            ],
-            verbose,
-        )
+
+def _torch_version() -> Optional[str]:
+    """The installed torch's version, None without one; torch itself is not imported for it."""
+    try:
+        return importlib.metadata.version("torch")
+    except importlib.metadata.PackageNotFoundError:
+        return None
+
+
+def _build_torch_module(force: bool, verbose: bool) -> None:
+    """libkge_torch, built anew for another torch than the one it was built for.  Without torch nobody can load it: nothing is built,
+    and the parts that need no torch stand by themselves."""
+    binding, version = CSRC / "torch_binding.cpp", _torch_version()
+    if version is None:
+        print("libkge_torch is not built: there is no torch", file=sys.stderr)
+        return
+    built_for = HERE / "build" / "libkge_torch.version"
+    same = built_for.exists() and built_for.read_text() == version
+    if not force and same and not _newer_than(TORCH_MODULE, [binding, INCLUDE / "kge_b200.h"]):
+        return
+    from torch.utils import cpp_extension
+
+    includes = [f"-I{p}" for p in cpp_extension.include_paths("cuda") + [sysconfig.get_paths()["include"], INCLUDE]]
+    torch_libs = [f"-L{p}" for p in cpp_extension.library_paths()]
+    _run(
+        [
+            os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-Wall", "-DTORCH_EXTENSION_NAME=libkge_torch", *includes,
+            binding, "-o", TORCH_MODULE, f"-L{HERE}", "-lkge_b200", *torch_libs, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10",
+            "-lc10_cuda", "-Wl,-rpath,$ORIGIN",
+        ],
+        verbose,
+    )
+    built_for.parent.mkdir(exist_ok=True)
+    built_for.write_text(version)
 
 
 if __name__ == "__main__":
