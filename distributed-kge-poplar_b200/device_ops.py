@@ -80,7 +80,7 @@ def _dequantise(self: Rows8) -> torch.Tensor:
     """The float32 values that the rows stand for."""
     blocks = -(-self.cols // BLOCK)
     # [row tile, group, row % 32, row / 32, block % 4] -> [row, block]
-    e = self.exponents.view(-(-self.rows // 128), -1, 32, 4, 4).permute(0, 3, 2, 1, 4).reshape(-(-self.rows // 128) * 128, -1)
+    e = self.exponents.view(-(-self.rows // 128), -(-blocks // 4), 32, 4, 4).permute(0, 3, 2, 1, 4).reshape(-(-self.rows // 128) * 128, -(-blocks // 4) * 4)
     e = e[: self.rows, :blocks].int()
     power = torch.where(e > 0, e << 23, 1 << 22).view(torch.float32)  # 2^-127 is a subnormal fp32
     return self.values.view(torch.float8_e4m3fn)[:, : self.cols].float() * power.repeat_interleave(BLOCK, 1)[:, : self.cols]

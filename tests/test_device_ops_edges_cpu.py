@@ -35,3 +35,14 @@ def test_a_product_that_gave_up_is_an_error(monkeypatch):
         device_ops.check_product8()
     monkeypatch.setattr(Library, "status", capi.OK)
     device_ops.check_product8()
+
+
+@pytest.mark.parametrize("rows,cols", [(0, 5), (0, 0), (3, 0), (2, 130)])
+def test_dequantised_rows_have_their_shape(rows, cols):
+    class Rows:  # what the values and their exponents lie in
+        values = torch.zeros(rows, -(-cols // 128) * 128 if cols > 128 else -(-cols // 16) * 16, dtype=torch.uint8)
+        exponents = torch.full((-(-rows // 128) * -(-cols // 512) * 512,), 127, dtype=torch.uint8)
+
+    Rows.rows, Rows.cols = rows, cols
+    got = device_ops.Rows8.dequantise(Rows)
+    assert got.shape == (rows, cols) and got.dtype == torch.float32 and torch.all(got == 0)
