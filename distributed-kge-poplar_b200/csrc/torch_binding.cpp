@@ -373,6 +373,20 @@ struct AdamWTensors {
 };
 
 std::pair<Tensor, Tensor> adamw_moments(const Tensor& adam_m, const Tensor& m_exponent, const Tensor& adam_v, const Tensor& v_exponent) {
+    // what an optimiser holds may have been replaced since it was made
+    const int64_t size = adam_m.numel();
+    const auto must_be = [&](const char* what, const Tensor& t, int64_t n) {
+        if (t.scalar_type() != at::kByte) refuse(what, " must be torch.uint8, not ", type_name(t.scalar_type()));
+        must_have_shape(what, t, {n});
+        if (!t.is_contiguous()) refuse(what, " must be contiguous");
+    };
+    must_be("m_exponent", m_exponent, size / 128);
+    must_be("v_exponent", v_exponent, size / 128);
+    must_be("adam_v", adam_v, size);
+    must_be("adam_m", adam_m, size);
+    must_be_with("m_exponent", m_exponent, adam_m.device());
+    must_be_with("v_exponent", v_exponent, adam_m.device());
+    must_be_with("adam_v", adam_v, adam_m.device());
     const c10::cuda::CUDAGuard guard(adam_m.device());
     const auto type = adam_m.options().dtype(at::kBFloat16);
     Tensor m = at::empty(adam_m.sizes(), type), v = at::empty(adam_m.sizes(), type);

@@ -46,3 +46,14 @@ def test_dequantised_rows_have_their_shape(rows, cols):
     Rows.rows, Rows.cols = rows, cols
     got = device_ops.Rows8.dequantise(Rows)
     assert got.shape == (rows, cols) and got.dtype == torch.float32 and torch.all(got == 0)
+
+
+def test_moments_that_do_not_fit_one_another():
+    def bytes_(n):
+        return torch.zeros(n, dtype=torch.uint8)
+
+    for moments, text in [((bytes_(256), bytes_(1), bytes_(256), bytes_(2)), "m_exponent has shape"), ((bytes_(256), bytes_(2), bytes_(256), bytes_(1)), "v_exponent has shape"),
+                          ((bytes_(256), bytes_(2).float(), bytes_(256), bytes_(2)), "m_exponent must be torch.uint8"),
+                          ((bytes_(256), bytes_(4)[::2], bytes_(256), bytes_(2)), "m_exponent must be contiguous"), ((bytes_(256), bytes_(2), bytes_(256), bytes_(2)), "on a GPU")]:
+        with pytest.raises(ValueError, match=text):
+            device_ops._module.adamw_moments(*moments)

@@ -223,3 +223,15 @@ def test_a_schedule_is_written_without_waiting(ops):  # noqa: F811
         with torch.cuda.graph(torch.cuda.CUDAGraph()):
             other.advance(schedule, 0.01)
     assert other.step_count == 21
+
+
+def test_moments_whose_memory_was_replaced(ops):  # noqa: F811
+    for name, text in [("m_exponent", "m_exponent has shape"), ("v_exponent", "v_exponent has shape"), ("adam_v", "adam_v has shape"), ("adam_m", "exponent has shape")]:
+        optimiser = ops.AdamW([torch.zeros(400).cuda()], state_bits=8)
+        kept = getattr(optimiser, name)
+        setattr(optimiser, name, kept[: kept.numel() // 2])
+        with pytest.raises(ValueError, match=text):
+            optimiser.moments()
+        setattr(optimiser, name, kept.cpu())
+        with pytest.raises(ValueError, match="on a GPU|is on"):
+            optimiser.moments()
