@@ -19,6 +19,7 @@ from __future__ import annotations
 
 import contextlib
 import importlib.util
+import operator
 from pathlib import Path
 from typing import Any, Dict, Optional, Sequence, Tuple, Union
 
@@ -208,11 +209,19 @@ class AdamW:
         return dict(step_count=self.step_count, seed=self.seed, **{name: getattr(self, name).clone() for name in self._state_names()})
 
     def load_state(self, state: Dict[str, Any]) -> None:
-        """Sets what :meth:`state` gave for an optimiser of the same tensors and state_bits."""
+        """Sets what :meth:`state` gave for an optimiser of the same tensors and state_bits.  One that does not fit changes nothing."""
         for name in self._state_names():
             mine, given = getattr(self, name), state.get(name)
-            if given is None or given.shape != mine.shape or given.dtype != mine.dtype:
+            if not isinstance(given, torch.Tensor) or given.shape != mine.shape or given.dtype != mine.dtype:
                 raise ValueError(f"'{name}' of the state does not fit this optimiser")
+        numbers = {}
+        for name in ("step_count", "seed"):
+            try:
+                numbers[name] = operator.index(state.get(name))
+            except TypeError:
+                raise ValueError(f"'{name}' of the state does not fit: {state.get(name)!r}") from None
+        if numbers["step_count"] < 0:
+            raise ValueError(f"'step_count' of the state does not fit: {numbers['step_count']}")
         for name in self._state_names():
             getattr(self, name).copy_(state[name])
-        self.step_count, self.seed = int(state["step_count"]), int(state["seed"])
+        self.step_count, self.seed = numbers["step_count"], numbers["seed"] & 0xFFFFFFFF

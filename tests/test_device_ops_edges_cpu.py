@@ -57,3 +57,28 @@ def test_moments_that_do_not_fit_one_another():
                           ((bytes_(256), bytes_(4)[::2], bytes_(256), bytes_(2)), "m_exponent must be contiguous"), ((bytes_(256), bytes_(2), bytes_(256), bytes_(2)), "on a GPU")]:
         with pytest.raises(ValueError, match=text):
             device_ops._module.adamw_moments(*moments)
+
+
+def optimiser_of(bits, total=256):
+    """An optimiser as it is between its calls, without the GPU that its construction asks for."""
+    optimiser = object.__new__(device_ops.AdamW)
+    optimiser.state_bits, optimiser.step_count, optimiser.seed, optimiser.device = bits, 3, 7, torch.device("cpu")
+    kind = torch.float32 if bits == 32 else torch.uint8
+    optimiser.adam_m, optimiser.adam_v = torch.zeros(total, dtype=kind), torch.zeros(total, dtype=kind)
+    optimiser.m_exponent, optimiser.v_exponent = torch.zeros(total // 128, dtype=torch.uint8), torch.zeros(total // 128, dtype=torch.uint8)
+    return optimiser
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_state_that_does_not_fit_changes_nothing(bits):
+    optimiser, other = optimiser_of(bits), optimiser_of(bits)
+    for t in (other.adam_m, other.adam_v):
+        t.fill_(5)
+    whole = other.state()
+    for change in (dict(step_count=None), dict(step_count=-1), dict(step_count=1.5), dict(seed=None), dict(seed="x"), dict(adam_v=whole["adam_v"][:128]), dict(adam_v=[5] * 256)):
+        for state in (dict(whole, **change), {k: v for k, v in whole.items() if k not in change}):
+            with pytest.raises(ValueError, match="does not fit"):
+                optimiser.load_state(state)
+            assert torch.all(optimiser.adam_m == 0) and torch.all(optimiser.adam_v == 0) and (optimiser.step_count, optimiser.seed) == (3, 7)
+    optimiser.load_state(dict(whole, step_count=torch.tensor(9), seed=-1))
+    assert torch.all(optimiser.adam_m == 5) and (optimiser.step_count, optimiser.seed) == (9, 0xFFFFFFFF)
