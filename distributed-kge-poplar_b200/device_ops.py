@@ -158,8 +158,11 @@ class AdamW:
                 _module.adamw_key(self.seed, step & 0xFFFFFFFF))
 
     def new_schedule(self) -> torch.Tensor:
-        """Device memory for :meth:`advance`, read by steps that are captured into a graph."""
-        return torch.zeros(4, dtype=torch.float32, device=self.device)
+        """Device memory for :meth:`advance`, read by steps that are captured into a graph.  Until it is advanced it is that of a step of
+        length 0: moments are updated, parameters stay."""
+        schedule = torch.zeros(4, dtype=torch.float32, device=self.device)
+        schedule[:1] = schedule[2:3] = 1.0  # decay and the second moments' correction
+        return schedule
 
     def advance(self, schedule: torch.Tensor, learning_rate: float) -> None:
         """Counts a step and writes what it needs into ``schedule``, on the current stream: before each replay of a graph that holds

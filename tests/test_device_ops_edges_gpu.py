@@ -235,3 +235,13 @@ def test_moments_whose_memory_was_replaced(ops):  # noqa: F811
         setattr(optimiser, name, kept.cpu())
         with pytest.raises(ValueError, match="on a GPU|is on"):
             optimiser.moments()
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_schedule_that_was_not_advanced_leaves_the_parameters(ops, dtype, bits):  # noqa: F811
+    start = torch.randn(1000, generator=gen(8)).to(dtype)
+    p = start.cuda()
+    optimiser = ops.AdamW([p], state_bits=bits)
+    optimiser.step([torch.randn(1000, generator=gen(9)).to(dtype).cuda()], schedule=optimiser.new_schedule())  # as a step before a capture may be
+    assert torch.equal(p.cpu(), start)
