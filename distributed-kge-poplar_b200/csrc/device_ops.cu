@@ -258,7 +258,10 @@ void launch_product(const CUtensorMap& a, const CUtensorMap& b, rows8::ProductAr
         if (g.blocks <= Kept::kMostResident && g.splits == 1 && g.m_tiles <= kSmCount) {
             CUtensorMap out = b;  // where results are stored directly, any map
             g.stages = Kept::lone_stages(g.blocks);
-            g.boxes = TM >= 64 && aligned_to(g.out, 16) && (g.m == 1 || g.out_stride * (long long)sizeof(TOut) % 16 == 0);
+            // A box that ends inside 16 bytes of a row is written to their end, past the row's columns: where the rows' width is no multiple
+            // of 16 bytes the last tile is stored directly.
+            if (TM >= 64 && aligned_to(g.out, 16) && (g.m == 1 || g.out_stride * (long long)sizeof(TOut) % 16 == 0))
+                g.boxes = (size_t)g.n * sizeof(TOut) % 16 == 0 ? g.n_tiles : g.n / rows8::kTileN;
             if (g.boxes)
                 out = encoded_map(map_type<TOut>(), g.out, (cuuint64_t)g.n, (cuuint64_t)g.m, round_up((size_t)std::max<long long>(g.out_stride, g.n) * sizeof(TOut), 16),
                                   rows8::kBoxColumns<TOut>, rows8::kBoxRows<TOut>, sizeof(TOut) == 4 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B);

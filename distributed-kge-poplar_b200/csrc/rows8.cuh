@@ -314,7 +314,7 @@ struct ProductArgs {
     int n_tiles, m_tiles, splits;
     int chunk;  // tiles of n that are gone through for all of m before the next ones
     int stages; // of the ring
-    int boxes;  // 1: `out` takes whole boxes of a tile's rows
+    int boxes;  // tiles of n whose results go out as boxes of a tile's rows
 };
 
 // The tiles of a block, one after another.  Tiles that are worked on at the same time lie side by side along the rows of `out`, so
@@ -714,17 +714,15 @@ k_product8(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CU
                 }
                 if (ended) break;
                 TOut* const out = static_cast<TOut*>(g.out) + (long long)m0 * g.out_stride + n0 + lane;
+                const bool boxed = tile.nt < g.boxes;  // the others come last: a block's tiles go up
 #pragma unroll
                 for (int i = 0; i < kChunks; ++i) {
                     const int rows = min(kRows, g.m - m0 - 32 * i);
                     if (rows <= 0) break;  // the same for the four warps
                     if constexpr (kTurn) {
-                        if (g.boxes) {
-                            if (issues) box_stores_read();
-                            two_warps_sync(pair);
-                        } else {
-                            four_warps_sync(part);  // the rows before have been read
-                        }
+                        if (issues && g.boxes) box_stores_read();
+                        if (boxed) two_warps_sync(pair);
+                        else four_warps_sync(part);  // the rows before have been read
 #pragma unroll
                         for (int q = 0; q < 4; ++q) {  // eight rows of `out` each, of 16 bytes for each eight lanes
                             const uint32_t at = tc::smem_u32(box) + (q * 8 + (lane & 7)) * 128 + (((quad % 2 * 4 + lane / 8) ^ (lane & 7)) << 4);
@@ -732,7 +730,7 @@ k_product8(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CU
                             const float* const hi = acc[i] + 16 + 4 * q;
                             store_turned(at, rounded_pair<TOut>(lo[0], lo[1]), rounded_pair<TOut>(lo[2], lo[3]), rounded_pair<TOut>(hi[0], hi[1]), rounded_pair<TOut>(hi[2], hi[3]));
                         }
-                        if (g.boxes) {
+                        if (boxed) {
                             tc::fence_async_shared();
                             two_warps_sync(pair);
                             if (issues && n0 < g.n) box_store(&out_map, box, n0, m0 + 32 * i);
@@ -741,7 +739,7 @@ k_product8(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CU
                             store_rows(boxes + part * 2 * L::kBoxBytes, static_cast<TOut*>(g.out) + (long long)(m0 + 32 * i) * g.out_stride + tile.nt * kTileN, g.out_stride,
                                        quad * 8, min(rows, quad * 8 + 8), min(kTileN, g.n - tile.nt * kTileN));
                         }
-                    } else if (TM >= 64 && g.boxes) {
+                    } else if (TM >= 64 && boxed) {
 #pragma unroll
                         for (int h = 0; h < 32; h += kBoxRows<TOut>) {
                             if (h >= rows) break;

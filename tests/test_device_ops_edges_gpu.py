@@ -9,7 +9,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 import device_op_forms as forms  # noqa: E402
-from test_device_ops_gpu import TYPES, U, check_log_probs, cuda, gen, grad_tolerance, log_tolerance, ops  # noqa: E402, F401
+from test_device_ops_gpu import TYPES, U, check_log_probs, cuda, gen, grad_tolerance, log_tolerance, ops, product_tolerance, rows_of_lengths  # noqa: E402, F401
 
 pytestmark = pytest.mark.gpu
 
@@ -245,3 +245,20 @@ def test_a_schedule_that_was_not_advanced_leaves_the_parameters(ops, dtype, bits
     optimiser = ops.AdamW([p], state_bits=bits)
     optimiser.step([torch.randn(1000, generator=gen(9)).to(dtype).cuda()], schedule=optimiser.new_schedule())  # as a step before a capture may be
     assert torch.equal(p.cpu(), start)
+
+
+@pytest.mark.parametrize("n", [1, 7, 77, 127, 129, 300, 385, 1001])
+@pytest.mark.parametrize("m", [20, 40, 100, 300])
+def test_product8_into_a_part_of_rows_on_16_bytes(ops, m, n):  # noqa: F811
+    """Results of any width in rows that begin on 16 bytes: what lies beside and below them stays."""
+    k = 130
+    a, b = (ops.quantise_rows(rows_of_lengths(rows, k, rows).clamp(-1e3, 1e3).cuda()) for rows in (m, n))
+    for out in TYPES:
+        want, tol = product_tolerance(a.dequantise().double(), b.dequantise().double(), k, out)
+        fine = want.abs() < 60000 if out == torch.float16 else torch.ones_like(want, dtype=torch.bool)
+        for lead in (0, 8):
+            frame = torch.full((m + 3, n + 16 + -n % 8), 5.0, dtype=out, device="cuda")
+            got = ops.product8(a, b, out=frame[:m, lead : lead + n])
+            assert torch.all(((got.double() - want).abs() <= tol) | ~fine)
+            frame[:m, lead : lead + n] = 5
+            assert torch.all(frame == 5)
