@@ -262,3 +262,85 @@ def test_product8_into_a_part_of_rows_on_16_bytes(ops, m, n):  # noqa: F811
             assert torch.all(((got.double() - want).abs() <= tol) | ~fine)
             frame[:m, lead : lead + n] = 5
             assert torch.all(frame == 5)
+
+
+# (queries, rows of the table, values of a row): a block's tile of 16, 32, 64, 128 or 256 queries, which it keeps or fetches with each part
+# of the table; more tiles than blocks; tiles in a row or four side by side; sums of one to four times 2048 values.
+MANY_TILES = [(100, 25_001, 256), (512, 10_003, 300), (1500, 7000, 200), (600, 7700, 900), (513, 3205, 2100), (300, 9600, 6200), (100, 20_001, 900),
+              (64, 20_000, 1700), (20, 20_001, 3300), (9, 20_003, 6500), (19_001, 300, 100)]
+
+
+@pytest.mark.parametrize("m,n,k", MANY_TILES)
+def test_product8_of_many_tiles(ops, m, n, k):  # noqa: F811
+    g = torch.Generator(device="cuda").manual_seed(m + n + k)
+
+    def rows(count):
+        length = torch.exp(2 * torch.randn(count, 1, generator=g, device="cuda"))
+        return (torch.randn(count, k, generator=g, device="cuda") * length).clamp(-1e3, 1e3)
+
+    a, b = ops.quantise_rows(rows(m)), ops.quantise_rows(rows(n))
+    for out in TYPES:
+        want, tol = product_tolerance(a.dequantise().double(), b.dequantise().double(), k, out)
+        fine = want.abs() < 60000 if out == torch.float16 else torch.ones_like(want, dtype=torch.bool)
+        for pad, lead in ((0, 0), (9, 3), (8 - n % 8, 0)):  # as it comes, at no boundary, in rows on 16 bytes
+            frame = torch.full((m + 2, n + pad), 5.0, dtype=out, device="cuda")
+            got = ops.product8(a, b, out=frame[:m, lead : lead + n])
+            off = (got.double() - want).abs()
+            assert torch.all((off <= tol) | ~fine), (out, pad, (off / tol)[fine].max())
+            assert torch.all(frame[:m, :lead] == 5) and torch.all(frame[:m, lead + n :] == 5) and torch.all(frame[m:] == 5)
+    ops.check_product8()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("size", SHAPES)
+def test_masks_and_counts_in_every_size_of_block(ops, size, dtype):  # noqa: F811
+    """What is hidden holds NaN, infinities and numbers above all others; some rows are hidden whole, some columns in all rows."""
+    rows, cols = SHAPES[size]
+    g, scale = gen(cols + 2), 0.7
+    x = (torch.randn(rows, cols, generator=g) * 3).to(dtype)
+    mask = torch.rand(rows, cols, generator=g) > 0.4
+    mask[:, cols // 3 : cols // 2] = False
+    mask[2::7] = False
+    count = torch.randint(1, cols + 9, (rows,), generator=g, dtype=torch.int32)
+    target = torch.randint(-1, cols, (rows,), generator=g, dtype=torch.int32)
+    live = forms.live_columns(x, mask, count)
+    hidden = torch.where(live, x, torch.tensor([math.nan, math.inf, -math.inf, 6e4])[torch.arange(cols) % 4].to(dtype)).cuda()
+    weights = [torch.randn(shape, generator=g) for shape in ((rows,), (rows,), (rows, 40))]
+    want = forms.log_probs(x, target, mask, count, scale=scale, n_best=40)
+    right = forms.log_probs_grad(x, want, target, scale, *weights)
+    tol = grad_tolerance(want, dtype, weights[0].double().abs() + weights[2].double().abs().sum(1), weights[1].double(), scale, cols, right)
+    wide = torch.zeros(rows, cols + 5, dtype=torch.bool).cuda()  # a mask at no boundary
+    wide[:, 3 : cols + 3] = mask.cuda()
+    for m in (mask.cuda(), wide[:, 3 : cols + 3]):
+        got = ops.log_probs(hidden, target.cuda(), mask=m, count=count.cuda(), scale=scale, n_best=40)
+        check_log_probs(got, want, cols)
+        grad = ops.log_probs_grad(hidden, got, grad_log_prob=weights[0].cuda(), grad_entropy=weights[1].cuda(), grad_best=weights[2].cuda()).cpu().double()
+        assert torch.all(grad[~live] == 0) and torch.all((grad - right).abs() <= tol), ((grad - right).abs() / tol).nan_to_num(0).max()
+
+
+@pytest.mark.parametrize("grad_type", TYPES)
+@pytest.mark.parametrize("param_type", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_of_tensors_at_no_boundary(ops, bits, param_type, grad_type):  # noqa: F811
+    """Draws depend on a value's place in the moments alone: tensors that lie elsewhere get the same bits."""
+    sizes, g = [1, 5, 127, 128, 513, 2000, 16, 700], gen(21)
+    start = [torch.randn(n, generator=g).to(param_type) for n in sizes]
+
+    def lying(values, lead):
+        held = [torch.full((len(v) + lead + 3,), 7.0, dtype=v.dtype).cuda() for v in values]
+        for h, v in zip(held, values):
+            h[lead : lead + len(v)] = v.cuda()
+        return held, [h[lead : lead + len(v)] for h, v in zip(held, values)]
+
+    kept = [lying(start, lead) for lead in (0, 1, 2, 4)]
+    optimisers = [ops.AdamW(views, state_bits=bits, seed=11, weight_decay=0.1) for _, views in kept]
+    for _ in range(3):
+        grads = [(torch.randn(n, generator=g) * torch.exp(torch.randn(n, generator=g))).to(grad_type) for n in sizes]
+        for i, optimiser in enumerate(optimisers):
+            optimiser.step(lying(grads, (0, 1, 2, 4)[i])[1], 0.01)
+    for (held, views), optimiser, lead in zip(kept[1:], optimisers[1:], (1, 2, 4)):
+        for h, v, w in zip(held, views, kept[0][1]):
+            assert torch.equal(v, w) and not torch.equal(v, start[0].cuda())
+            assert torch.all(h[:lead] == 7) and torch.all(h[lead + len(v) :] == 7)
+        for name in optimiser._state_names():
+            assert torch.equal(getattr(optimiser, name), getattr(optimisers[0], name))
