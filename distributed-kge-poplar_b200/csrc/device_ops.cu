@@ -205,6 +205,9 @@ void quantise_rows(const void* x, int float_type, size_t rows, size_t cols, long
 
 namespace {
 
+// Sizes whose plan is counted in ints: others are refused, and want no workspace.
+bool product_fits(size_t m, size_t n, size_t k) { return m <= 0x7fffffffu && n <= 0x7fffffffu - 65536 && k <= 0x7fffffffu - 65536; }
+
 struct ProductPlan {
     int tile_m, m_tiles, n_tiles, blocks, splits, chunk;
 };
@@ -284,7 +287,7 @@ void launch_product(int tile_m, const CUtensorMap& a, const CUtensorMap& b, cons
 }  // namespace
 
 size_t product8_workspace(size_t m, size_t n, size_t k) {
-    if (m == 0 || n == 0 || k == 0 || m > 0x7fffffffu || n > 0x7fffffffu) return 0;
+    if (m == 0 || n == 0 || k == 0 || !product_fits(m, n, k)) return 0;
     const ProductPlan p = product_plan(m, n, k);
     return p.splits > 1 ? (size_t)p.splits * m * n * sizeof(float) : 0;
 }
@@ -293,7 +296,7 @@ void product8(const uint8_t* a_values, const uint8_t* a_exponents, size_t m, con
               size_t k, void* out, int out_type, long long out_row_stride, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
     const char* const what = "kge_op_product8";
     const size_t bytes = type_bytes(out_type, what);
-    if (m > 0x7fffffffu || n > 0x7fffffffu - 65536 || k > 0x7fffffffu - 65536) fail(KGE_INVALID_ARGUMENT, msg() << what << ": " << m << " x " << n << " x " << k << " is too large");
+    if (!product_fits(m, n, k)) fail(KGE_INVALID_ARGUMENT, msg() << what << ": " << m << " x " << n << " x " << k << " is too large");
     if (m > 1 && out_row_stride < (long long)n) fail(KGE_INVALID_ARGUMENT, msg() << what << ": rows of " << n << " results, " << out_row_stride << " apart");
     if (m == 0 || n == 0) return;
     need(out, "kge_op_product8: null output");

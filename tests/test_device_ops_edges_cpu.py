@@ -5,7 +5,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 from distributed_kge_poplar_b200 import capi, device_ops  # noqa: E402
-from test_device_ops_cpu import adamw, refused  # noqa: E402
+from test_device_ops_cpu import SOME, adamw, lib, refused  # noqa: E402
 
 
 @pytest.mark.parametrize("epsilon", [0.0, -1e-8, 1e-46, 1e-39, float("nan"), float("inf"), 1e39])
@@ -82,3 +82,10 @@ def test_a_state_that_does_not_fit_changes_nothing(bits):
             assert torch.all(optimiser.adam_m == 0) and torch.all(optimiser.adam_v == 0) and (optimiser.step_count, optimiser.seed) == (3, 7)
     optimiser.load_state(dict(whole, step_count=torch.tensor(9), seed=-1))
     assert torch.all(optimiser.adam_m == 5) and (optimiser.step_count, optimiser.seed) == (9, 0xFFFFFFFF)
+
+
+def test_workspaces_of_sizes_that_are_refused():
+    for k in (2**31, 2**38, 2**57, 2**64 - 1):
+        assert lib.kge_op_product8_workspace(4, 8, k) == 0
+        refused(lib.kge_op_product8(SOME, SOME, 4, SOME, SOME, 8, k, SOME, capi.F32, 8, SOME, 2**40, None), "too large")
+    assert lib.kge_op_product8_workspace(2**31 - 1, 2**31 - 1, 2**31) == 0
