@@ -365,10 +365,11 @@ struct AdamWTensors {
             a.schedule = schedule->data_ptr<float>();
         }
         must_not_meet(c10::elementSize(*grad_type));
+        // as any operator that writes in place tells autograd; it may refuse (tensors of inference mode), so it comes first
+        for (size_t i = 0; i < params.size(); ++i)
+            if (table[i].size) params[i].unsafeGetTensorImpl()->bump_version();
         const c10::cuda::CUDAGuard guard(device);
         check(kge_op_adamw(&a, table.data(), table.size(), stream_of(device)));
-        for (size_t i = 0; i < params.size(); ++i)
-            if (table[i].size) params[i].unsafeGetTensorImpl()->bump_version();  // as any operator that writes in place tells autograd
     }
 };
 

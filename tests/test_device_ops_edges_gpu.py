@@ -344,3 +344,15 @@ def test_adamw_of_tensors_at_no_boundary(ops, bits, param_type, grad_type):  # n
             assert torch.all(h[:lead] == 7) and torch.all(h[lead + len(v) :] == 7)
         for name in optimiser._state_names():
             assert torch.equal(getattr(optimiser, name), getattr(optimisers[0], name))
+
+
+def test_parameters_of_inference_mode(ops):  # noqa: F811
+    """Stepped there; outside they may not be written, by torch's operators neither, and are not."""
+    with torch.inference_mode():
+        p = torch.zeros(300).cuda()
+        optimiser = ops.AdamW([p])
+        optimiser.step([torch.ones(300).cuda()], 0.1)
+    after = p.cpu().clone()
+    with pytest.raises(RuntimeError, match="inference"):
+        optimiser.step([torch.ones(300).cuda()], 0.1)
+    assert torch.all(after < 0) and torch.equal(p.cpu(), after) and optimiser.step_count == 1
