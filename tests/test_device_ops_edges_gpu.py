@@ -356,3 +356,39 @@ def test_parameters_of_inference_mode(ops):  # noqa: F811
     with pytest.raises(RuntimeError, match="inference"):
         optimiser.step([torch.ones(300).cuda()], 0.1)
     assert torch.all(after < 0) and torch.equal(p.cpu(), after) and optimiser.step_count == 1
+
+
+def test_sizes_past_32_bits(ops):  # noqa: F811
+    """More than 2^31 scores, table values, results and parameters: the last rows are the same as by themselves."""
+    rows, cols, k = 21_600, 100_003, 16
+    g = torch.Generator(device="cuda").manual_seed(3)
+    queries, table = (torch.randn(n, k, generator=g, device="cuda") for n in (rows, cols))
+    table8 = ops.quantise_rows(table)
+    scores = ops.product8(queries, table8, dtype=torch.bfloat16)
+    assert scores.numel() > 2**31
+    last = slice(rows - 130, rows)
+    assert torch.equal(scores[last], ops.product8(queries[last].contiguous(), table8, dtype=torch.bfloat16))
+    target = torch.randint(cols, (rows,), generator=g, device="cuda", dtype=torch.int32)
+    mask = torch.ones(rows, cols, dtype=torch.bool, device="cuda")
+    mask[:, ::3] = False
+    result = ops.log_probs(scores, target, mask=mask, n_best=5)
+    few = ops.log_probs(scores[last], target[last].contiguous(), mask=mask[last], n_best=5)
+    tol = log_tolerance(cols, few.best_log_prob.double())
+    assert torch.equal(result.best_index[last], few.best_index) and torch.all((result.best_log_prob[last] - few.best_log_prob).abs() <= tol)
+    turned = ops.quantise_rows(scores, transposed=True)
+    part = ops.quantise_rows(scores[rows // 128 * 128 :], transposed=True)  # the blocks from there on
+    assert torch.equal(turned.values[:, rows // 128 * 128 : rows // 128 * 128 + part.values.shape[1]], part.values)
+    straight = ops.quantise_rows(scores)
+    assert torch.equal(straight.values[last], ops.quantise_rows(scores[last]).values)
+    weight = torch.full((rows,), -1.0, device="cuda")
+    grad = ops.log_probs_grad(scores[last].clone(), few, grad_log_prob=weight[last].contiguous())
+    ops.log_probs_grad(scores, result, grad_log_prob=weight, out=scores)
+    assert torch.all((scores[last].float() - grad.float()).abs() <= 2.0**-7 * grad.float().abs() + 1e-30)  # a neighbouring bf16 number at most
+    assert torch.all(scores[last][~mask[last]] == 0)
+    del turned, straight, mask, grad
+    p = torch.zeros(2**31 + 1000, dtype=torch.bfloat16, device="cuda")
+    optimiser = ops.AdamW([p[: 2**31 - 128], p[2**31 - 128 :]], state_bits=8)
+    optimiser.step([torch.ones_like(v) for v in optimiser.params], 0.25)
+    m, v = optimiser.moments()
+    for at in (slice(0, 1000), slice(2**31 - 1000, 2**31 + 1000)):
+        assert torch.all((p[at].float() + 0.25).abs() <= 2.0**-8) and torch.all((m[at].float() - 0.1).abs() <= 0.1 / 8) and torch.all((v[at].float() - 0.001).abs() <= 0.001 / 8)
