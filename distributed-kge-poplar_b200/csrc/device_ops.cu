@@ -64,12 +64,16 @@ lp::Scores checked_scores(const kge_scores& s, const char* what) {
 
 namespace {
 
-// A row is one block's, of as many threads as give each SM 1024: 128 rows of 100 003 bf16 scores with lists of 100 take 16 us by blocks
-// of 1024 threads, and in parts of 256 with a second kernel to join them 29.  Rows are cut into parts, four to an SM, where there are too
-// few of them for that or the groups of vectors of their lists do not fit a block's shared memory; two to an SM with lists, which each part
-// makes (4 rows of 2 500 001 fp32 scores 24.6 us, with four to an SM 26.0, by one block a row 713).  Many short rows go to blocks of 128
-// threads, whose sums are joined sooner: 4096 rows of 10 001 bf16 scores 26.8 us, by blocks of 256 33.1, with lists of 10 41.3 and 63.5;
-// 4096 of 20 001 fp32 ones, 5001 vectors each, take 62 us either way.
+// A row is one block's.  Each kernel holds 64 registers a thread, 1024 threads to an SM, and blocks are as large as leaves all rows at work
+// at once: 1024 threads for a row an SM, 512 for two.  A row more than that waits for a second, nearly empty wave, and smaller blocks are
+// sooner done: of 20 001 bf16 scores 148 rows 6.7 us by blocks of 1024; 149 11.5, by 512 5.4; with lists of 100 13.1; 21.1, by 512
+// 11.5; 297 rows by 512 8.2, by 256 7.9; of 100 003 bf16 scores with lists of 100 148 rows 18.0 by 1024; 149 30.5, by 512 20.4.
+// (128 rows of those in parts of 256 threads, with a second kernel to join them: 31.0, as rows of one block each 17.7.)
+// Rows are cut into parts, four to an SM, where there are too few of them for that (4 rows of 2 500 001 fp32 scores 12.1 us, by one block a
+// row 162; 60 of 200 001 bf16 ones 11.1, 16.2) or the groups of vectors of their lists do not fit a block's shared memory; two to an SM with
+// lists, which each part makes (4 rows with lists of 100 28.5, with four to an SM 30.3).  Many short rows go to blocks of 128 threads, whose
+// sums are joined sooner: 4096 rows of 10 001 bf16 scores 23.6 us, by blocks of 256 31.0, with lists of 10 39.3 and 60.6; 4096 of
+// 20 001 fp32 ones, 5001 vectors each, take 59.6 us either way.
 struct LogProbsPlan {
     int threads, parts, vectors;
     size_t sums_bytes, bytes;
@@ -85,7 +89,7 @@ LogProbsPlan log_probs_plan(size_t rows, size_t cols, size_t n_best, size_t widt
     if (all <= 512 || (rows >= 4 * kSmCount && all <= (n_best ? most(128) : 4096))) {
         p.threads = 128;
     } else {
-        p.threads = rows <= kSmCount + 12 ? 1024 : rows <= 2 * kSmCount + 24 ? 512 : 256;
+        p.threads = rows <= kSmCount ? 1024 : rows <= 2 * kSmCount ? 512 : 256;
         while (p.threads > 256 && (size_t)p.threads * 2 > all) p.threads /= 2;  // two vectors a thread at least
         if ((n_best && all > most(p.threads)) || (rows <= kSmCount / 2 && (all > 16384 || (rows <= 16 && all >= 2048)))) {
             p.threads = 256;
