@@ -318,8 +318,10 @@ struct ProductArgs {
 };
 
 // The tiles of a block, one after another.  Tiles that are worked on at the same time lie side by side along the rows of `out`, so
-// that its memory is written in long pieces (4096 x 62 500 bf16 results of 128-wide rows by 64 bytes of a row: 239 us, with neighbours
-// one above the other 294), in chunks whose part of the table stays in L2 until all of m has met it.  A block that keeps its rows of `a` goes along them.
+// that its memory is written in long pieces, in chunks whose part of the table stays in L2 until all of m has met it.  A block that keeps
+// its rows of `a` goes along them.  Where few blocks work on a row of `out` each does four tiles side by side (4736 queries, four blocks a row,
+// x 62 504 x 128 to bf16: 154 us, one tile at a time 232; eight blocks a row 77 and 79, nine 68 and 66, fourteen 53 and 50), if there
+// are tiles enough that none goes without (512 x 1387 x 256 to fp32, eleven tiles: 9.4 us by fours, one at a time 4.7).
 template <bool RESIDENT>
 struct Tiles {
     int w, step, n_work, stride, run;
@@ -330,7 +332,7 @@ struct Tiles {
             w = 0;
             step = 1;
             stride = (int)gridDim.x / g.m_tiles;
-            run = stride < 16 ? 4 : 1;  // where few blocks work on a row of `out`, each does four tiles side by side (292 -> 239 us)
+            run = stride <= 8 && g.n_tiles >= 16 * stride ? 4 : 1;
             n_work = (int)blockIdx.x < stride * g.m_tiles ? g.n_tiles : 0;
             split = 0;
         } else {

@@ -266,7 +266,7 @@ def test_product8_into_a_part_of_rows_on_16_bytes(ops, m, n):  # noqa: F811
 
 # (queries, rows of the table, values of a row): a block's tile of 16, 32, 64, 128 or 256 queries, which it keeps or fetches with each part
 # of the table; more tiles than blocks; tiles in a row or four side by side; sums of one to four times 2048 values.
-MANY_TILES = [(100, 25_001, 256), (512, 10_003, 300), (1500, 7000, 200), (600, 7700, 900), (513, 3205, 2100), (300, 9600, 6200), (100, 20_001, 900),
+MANY_TILES = [(100, 25_001, 256), (512, 10_003, 300), (1500, 7000, 200), (4700, 9001, 100), (600, 7700, 900), (513, 3205, 2100), (300, 9600, 6200), (100, 20_001, 900),
               (64, 20_000, 1700), (20, 20_001, 3300), (9, 20_003, 6500), (19_001, 300, 100)]
 
 
