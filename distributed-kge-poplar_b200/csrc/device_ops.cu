@@ -219,7 +219,7 @@ ProductPlan product_plan(size_t m, size_t n, size_t k) {
     ProductPlan p;
     p.n_tiles = (int)((n + rows8::kTileN - 1) / rows8::kTileN);
     p.tile_m = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : m <= 128 ? 128 : 256;
-    // Blocks that keep their queries have a tile's 128 (512 x 500 000 x 256: 125 us, with 256, whose accumulators share columns, 143);
+    // Blocks that keep their queries have a tile's 128 (512 x 500 000 x 256: 117 us, with 256, whose accumulators share columns, 148);
     // where the sum has to be split, smaller tiles need half the parts and so half the partial sums.
     if (p.tile_m == 256 && rows8::blocks_of(k) <= (size_t)rows8::Tile<128, true>::kMostResident && m <= (size_t)kSmCount * 128) p.tile_m = 128;
     if (p.tile_m == 256 && (long long)((m + 255) / 256) * p.n_tiles < kSmCount / 2) p.tile_m = 128;
@@ -369,6 +369,8 @@ void launch_adamw(const adamw::Table<adamw::kMaxTensors>& all, const adamw::Para
 }
 template <class TP, class TG>
 void launch_adamw(const adamw::Table<adamw::kMaxTensors>& all, const adamw::Params& p, const kge_adamw_args& a, cudaStream_t stream) {
+    // few tensors take a table of their own size along with the launch: a call with one 4.8 us, with six 5.2, in the large table's 10 KB 5.3
+    // and 5.6; captured steps do not see it
     if (all.n <= 16) launch_adamw<TP, TG, 16>(all, p, a, stream);
     else launch_adamw<TP, TG, adamw::kMaxTensors>(all, p, a, stream);
 }

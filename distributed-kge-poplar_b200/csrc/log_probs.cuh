@@ -626,9 +626,9 @@ struct Parts {
 // reference is one instruction, and off by half a unit of that product: from 2^31 on more than fp32 has exponents for.)  Scores are
 // raised to kLow first, so that -inf makes no NaN of e d; where the largest score is no further than 2^64 above kLow that would count
 // them, and add_exactly does the part again.
-// Reading bounds fp32 rows (1024 x 200 001: 133 us, 6.1 TB/s); of bf16 ones, twice the scores for the same bytes, the exponentials, 16 an SM
-// and cycle, take 45 of 82 us beside the reading's 62 (2048 x 100 001: 5.0 TB/s; 83.5 without the next four vectors under way and one
-// sum at a time).
+// Reading bounds fp32 rows (1024 x 200 001: 135 us, 6.1 TB/s; 132 without the next four vectors under way); of bf16 ones, twice the scores
+// for the same bytes, the exponentials, 16 an SM and cycle, take 45 of 80 us beside the reading's 62 (2048 x 100 001: 5.1 TB/s; 81.4
+// without the next four).
 template <int THREADS, class T>
 __device__ __forceinline__ Sums add_part(const Row<T>& row, int v0, int v1, float s2, float* groups, float& largest) {
     using W = Words<T>;
@@ -822,9 +822,8 @@ constexpr int kGradThreads = 256;
 
 // One block for kGradThreads * kGroup vectors of a row, the rows from the last to the first: what the forward pass read last may
 // still be in L2.  The vectors are those of the scores' memory: a gradient that is as far from a 16-byte boundary as the scores
-// are is written as it is read.  Bound by memory, it takes 144 us of 2048 x 100 001 bf16 scores and 156 of half as many fp32 ones (127 at
-// the copy rate); with registers for four blocks an SM 153 and 172, with two vectors a thread 164, for six blocks and a few spills 141
-// and 162.
+// are is written as it is read.  Bound by memory: 2048 x 100 001 bf16 scores 137 us, half as many fp32 ones 148 (127 at the copy rate).
+// Five blocks an SM serve both types: with registers for four 148 and 135, for six and a few spills 134 and 153.
 template <class T>
 static __global__ void __launch_bounds__(kGradThreads, 5) k_log_probs_grad(Scores s, GradArgs g) {
     constexpr int V = Row<T>::V;

@@ -6,7 +6,7 @@
 // tcgen05.mma.kind::mxf8f6f4.block_scale multiplies by a power of two per row and 32 values of k as it accumulates in fp32, so
 // a block's byte serves four instructions and nothing is left to do between them: the accumulator stays in TMEM over 2048 of k.
 //
-// What bounds it: the results' bytes where rows are short (512 x 500 000 x 256 to bf16, 512 MB: 125 us, 5.2 TB/s), the tensor cores
+// What bounds it: the results' bytes where rows are short (512 x 500 000 x 256 to bf16, 512 MB: 117 us, 5.5 TB/s with the table), the tensor cores
 // where they are long (8192 x 8192 x 4096: the product alone 2.6 PFLOP/s).
 #pragma once
 
@@ -398,7 +398,8 @@ struct Tile {
     static constexpr size_t smem() { return 1024 + (size_t)kSpace; }
 };
 // Where `out` takes boxes of whole lines: 64 columns of 16-bit results by 32 rows from two warps, 32 columns of fp32 by 16 rows from
-// one.  (4096 x 62 504 bf16 results of 128-wide rows: 146 us, stored 64 bytes of a row at a time 239.)
+// one.  (4096 x 62 504 bf16 results of 128-wide rows: 138 us, by words from shared memory 197; 512 x 500 000 of 256-wide ones 117 and
+// 174; 4096 x 62 504 fp32 ones 199, stored directly 208.)
 template <class TOut>
 constexpr int kBoxColumns = 128 / (int)sizeof(TOut);
 template <class TOut>
