@@ -247,7 +247,7 @@ def test_a_schedule_that_was_not_advanced_leaves_the_parameters(ops, dtype, bits
     assert torch.equal(p.cpu(), start)
 
 
-@pytest.mark.parametrize("n", [1, 7, 77, 127, 129, 300, 385, 1001])
+@pytest.mark.parametrize("n", [1, 7, 77, 127, 129, 264, 300, 385, 1001])
 @pytest.mark.parametrize("m", [20, 40, 100, 300])
 def test_product8_into_a_part_of_rows_on_16_bytes(ops, m, n):  # noqa: F811
     """Results of any width in rows that begin on 16 bytes: what lies beside and below them stays."""
@@ -311,7 +311,7 @@ def test_masks_and_counts_in_every_size_of_block(ops, size, dtype):  # noqa: F81
     tol = grad_tolerance(want, dtype, weights[0].double().abs() + weights[2].double().abs().sum(1), weights[1].double(), scale, cols, right)
     wide = torch.zeros(rows, cols + 5, dtype=torch.bool).cuda()  # a mask at no boundary
     wide[:, 3 : cols + 3] = mask.cuda()
-    for m in (mask.cuda(), wide[:, 3 : cols + 3]):
+    for m in (mask.cuda(), wide[:, 3 : cols + 3], mask.to(torch.uint8).cuda() * 130):
         got = ops.log_probs(hidden, target.cuda(), mask=m, count=count.cuda(), scale=scale, n_best=40)
         check_log_probs(got, want, cols)
         grad = ops.log_probs_grad(hidden, got, grad_log_prob=weights[0].cuda(), grad_entropy=weights[1].cuda(), grad_best=weights[2].cuda()).cpu().double()
