@@ -6,8 +6,8 @@
 // tcgen05.mma.kind::mxf8f6f4.block_scale multiplies by a power of two per row and 32 values of k as it accumulates in fp32, so
 // a block's byte serves four instructions and nothing is left to do between them: the accumulator stays in TMEM over 2048 of k.
 //
-// What bounds it: the results' bytes where rows are short (512 x 500 000 x 256 to bf16, 512 MB: 117 us, 5.5 TB/s with the table), the tensor cores
-// where they are long (8192 x 8192 x 4096: the product alone 2.6 PFLOP/s).
+// What bounds it: the results' bytes where rows are short (512 x 500 000 x 256 to bf16, 512 MB: 117 us, 5.5 TB/s with the table), the
+// tensor cores where they are long (8192 x 8192 x 4096: the product alone 2.6 PFLOP/s).
 #pragma once
 
 #include <cuda_bf16.h>
